@@ -222,6 +222,9 @@ def _prepare_pages(case, seed, g):
     state = {'case': case, 'lens': lens.to(DEV), 'table': table.to(DEV), 'refs': refs.to(DEV),
              'data': torch.randint(0, 256, (case['layers'], pages, case['bytes']), generator=g, device=DEV,
                                    dtype=torch.uint8)}
+    if own:
+        from xtier_amd import ops
+        state['buffers'] = ops.PageBuffers(list(state['data']))      # a server makes this once
     if case['path'] == 'fork':
         state['parents'] = torch.randint(0, live, (case['forks'],), generator=h, dtype=torch.int32).to(DEV)
         state['children'] = (live + torch.randperm(rows - live, generator=h)[:case['forks']]).int().to(DEV)
@@ -267,7 +270,7 @@ def _run_fork(s):
     if own:
         from xtier_amd import ops
         moves = ops.pages_fork(s['refs'], s['table'], s['lens'], s['parents'], s['children'], c['page'])
-        ops.pages_copy(list(s['data']), moves)
+        ops.pages_copy(s['buffers'], moves)
         forked = s['table'][s['children'].long()]
         ops.pages_free(s['refs'], s['table'], s['lens'], s['children'])
     else:
@@ -287,7 +290,7 @@ def _run_compact(s):
         ops.pages_free(s['refs'], s['table'], s['lens'], s['ended'])
         granted = ops.pages_extend(s['refs'], s['table'], s['lens'], s['add'], c['page'])
         moves, count = ops.pages_compact(s['refs'], s['table'])
-        ops.pages_copy(list(s['data']), moves, count)
+        ops.pages_copy(s['buffers'], moves, count)
     else:
         _plain_free(s['refs'], s['table'], s['lens'], s['ended'])
         granted = _plain_extend(s['refs'], s['table'], s['lens'], s['add'], c['page'])
