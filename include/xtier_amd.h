@@ -352,6 +352,117 @@ int xt_sparse_mla_fp8(const void* q, int64_t q_row_stride, int64_t q_head_stride
                       int64_t out_head_stride, int out_dtype, float* lse, int rows, int splits, void* workspace,
                       size_t workspace_bytes, xt_stream_t stream);
 
+/* --- the 8-bit paged cache ---------------------------------------------------------------------------------------- */
+
+/* No counterpart in the reference: a paged KV cache in E4M3 with one power-of-two scale for each page and KV head, for
+ * layers that attend to every key or to a sliding window. Page p, KV head h (byte strides; 0 = packed):
+ *   K block   k_pages + p * page_stride + h * head_stride: [page_size, dim] E4M3 bytes, token t's row at t * dim;
+ *   V block   vt_pages + the same offset: [dim, page_size] E4M3 bytes, transposed: dimension d of token t at
+ *             d * page_size + t;
+ *   scales    k_exp / v_exp + p * exp_page_stride + h * exp_head_stride: one byte e, the scale 2^(e - 127) (1..254).
+ * value = e4m3 * 2^(e - 127). page_size 16, 32, 64 or 128; dim 64, 128 or 256; blocks 16-byte aligned. Position j of
+ * request b lies in page table[b * table_stride + j / page_size] (int32, width columns), row j % page_size; a page id
+ * outside [0, pages) and a column past the width hold nothing.
+ *
+ * Requests: seq_lens[b] is request b's length with its new tokens; its rows of k / v or q are cu[b] .. cu[b + 1] - 1
+ * (int32 [batch + 1], not decreasing, cu[batch] <= rows; NULL: one row each, rows == batch), at the positions
+ * seq_lens[b] - n .. seq_lens[b] - 1 for n rows. A negative length counts as 0. */
+
+/* Quantize-on-append of K and V rows (BF16 [rows, kv_heads, dim], strides in elements, 16-byte aligned rows). For every
+ * page and head that takes rows, K and V alike:
+ *   need = the smallest e with max|x| <= 448 * 2^(e - 127) over the finite new values, kept within 63..246;
+ *   e = need if the page takes its first row (token 0) in this call: the page starts anew, and tokens that the call
+ *       does not write hold nothing; else max(need, the page's e);
+ *   new bytes = e4m3(x * 2^(127 - e)), to nearest even; beyond 448 (infinities) the largest value, NaN as NaN;
+ *   if e grew, the page's earlier tokens are rounded again: e4m3(old * 2^(old e - e)), which changes only values
+ *   that become subnormal.
+ * Bytes of later tokens stay as they are. Rows at negative positions, in a column past the table or in a page id
+ * outside the pool are skipped. No page may take rows of two requests in one call. */
+int xt_page8_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
+                    int64_t v_head_stride, int64_t rows, uint8_t* k_pages, uint8_t* vt_pages, uint8_t* k_exp,
+                    uint8_t* v_exp, int64_t pages, int kv_heads, int dim, int page_size, int64_t page_stride,
+                    int64_t head_stride, int64_t exp_page_stride, int64_t exp_head_stride, const int32_t* table,
+                    int64_t table_stride, int width, const int32_t* seq_lens, const int32_t* cu_rows, int batch,
+                    xt_stream_t stream);
+
+/* Device workspace of xt_page8_attention (0 on a bad argument). */
+size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_heads, int kv_heads, int dim);
+
+/* Attention over these pages, each query row causal at its own position p: query head h attends through KV head
+ * h / (q_heads / kv_heads) to the keys j <= p and, with window > 0, j > p - window or j < sinks (the first tokens stay
+ * visible), as far as pages hold them:
+ *   out[r, h] = sum_j softmax_j(q[r, h] . k_j * scale) v_j,   lse[r, h] = ln sum_j exp(q[r, h] . k_j * scale).
+ * Pages that no row sees (behind the window) may be freed: their table entries are not followed, or only to masked
+ * keys. Whatever hidden places hold, NaN included, changes nothing. A row that sees no key gives 0 and -inf; rows of q
+ * behind cu_q[batch] are left as they are. q: BF16 [rows, q_heads, dim] (strides in elements, 16-byte aligned rows);
+ * q_heads / kv_heads <= 128; scale > 0; out: out_dtype (strides in elements, 8-byte aligned rows); lse (optional): FP32
+ * [rows, q_heads]. QK exact products of BF16 with FP32 sums; P and V as FP16 in the second product (V exact within 15
+ * binades of scale below the largest of the row's pages), FP32 sums.
+ * workspace: xt_page8_attention_workspace_bytes bytes, 256-byte aligned, zero before its first use and left so where it
+ * has to be; calls of any shape may share one, one at a time. One launch on `stream`, its work divided on the device,
+ * so that a captured launch follows the lengths of each replay. */
+int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
+                       const uint8_t* vt_pages, const uint8_t* k_exp, const uint8_t* v_exp, int64_t pages, int kv_heads,
+                       int q_heads, int dim, int page_size, int64_t page_stride, int64_t head_stride,
+                       int64_t exp_page_stride, int64_t exp_head_stride, const int32_t* table, int64_t table_stride,
+                       int width, const int32_t* seq_lens, const int32_t* cu_q, int batch, int rows, int window,
+                       int sinks, float scale, void* out, int64_t out_row_stride, int64_t out_head_stride,
+                       int out_dtype, float* lse, void* workspace, size_t workspace_bytes, xt_stream_t stream);
+
+/* --- pages of a cache ---------------------------------------------------------------------------------------------- */
+
+/* No counterpart in the reference (its server keeps page tables on the host): bookkeeping of the pages that the caches
+ * of this library live in, on the device. refs int32 [pages]: how many table entries name a page, 0 for a free one;
+ * table int32 [rows, width] (row stride table_stride): the pages of each row's tokens in order, -1 behind them; lens
+ * int32 [rows]: tokens of each row, so that row b holds ceil(lens[b] / page_size) pages. Free pages are taken lowest
+ * first. Only full pages are ever shared, so a row may append to its last page. Rows, table entries and ids outside
+ * their range are left alone. page_size: a power of 2. */
+
+/* Device workspace of xt_pages_extend (forks 0), xt_pages_fork and xt_pages_compact (forks 0). */
+size_t xt_pages_workspace_bytes(int64_t pages, int forks);
+
+/* Each row b grows by add[b] >= 0 tokens: it gets the pages that ceil((lens[b] + add[b]) / page_size) columns need, and
+ * lens[b] += add[b]. Rows are served in order: a row whose pages, with those that the rows before it asked for, are more
+ * than the free ones gets none and keeps its length, and so does a row that would outgrow the table; granted[b]
+ * (uint8) says which grew. */
+int xt_pages_extend(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width, int32_t* lens,
+                    const int32_t* add, int rows, int page_size, uint8_t* granted, void* workspace,
+                    size_t workspace_bytes, xt_stream_t stream);
+
+/* Forks: row children[i] becomes a copy of row parents[i], sharing its full pages; an unfinished last page gets a free
+ * page of its own, dst, to which the caller copies src in every layer (xt_pages_copy): moves[i] = src,
+ * moves[moves_stride + i] = dst, both -1 where nothing is to be copied. Without a free page left (they are given in
+ * order) the child gets the full pages' tokens only. Lengths are those before the call. A fork is skipped if a row id is
+ * out of range, if the child holds tokens, or if an earlier fork of the call names the same child. forks <= 1024. */
+int xt_pages_fork(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width, int32_t* lens, int rows,
+                  int page_size, const int32_t* parents, const int32_t* children, int forks, int32_t* moves,
+                  int64_t moves_stride, void* workspace, size_t workspace_bytes, xt_stream_t stream);
+
+/* Frees rows which[0 .. n): every page of a row loses one reference, its table entries become -1 and its length 0. A
+ * row named twice is freed once. */
+int xt_pages_free(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width, int32_t* lens, int rows,
+                  const int32_t* which, int n, xt_stream_t stream);
+
+/* Compaction: with L pages in use, those at L and above move, in ascending order, to the free ones below L. refs and
+ * table follow; the caller copies the pages of every layer: moves[i] (from) and moves[pages / 2 + i] (to) for i <
+ * count[0] (at most pages / 2), -1 behind them. */
+int xt_pages_compact(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width, int rows,
+                     int32_t* moves, int32_t* count, void* workspace, size_t workspace_bytes, xt_stream_t stream);
+
+/* The pages of one buffer: page p holds `bytes` bytes at base + p * stride (copied 16 bytes at a time
+ * where base and stride are multiples of 16, else byte by byte). */
+typedef struct {
+  void* base;
+  int64_t pages, stride, bytes;
+} xt_page_buffer;
+#define XT_PAGES_COPY_MAX 64
+
+/* Copies page moves[i] to page moves[moves_stride + i] for i < n (and, with count, i < count[0]) in every buffer, in one
+ * launch; a move with an id outside a buffer's pages is skipped there. No destination may be another move's source or
+ * destination. n_buffers <= XT_PAGES_COPY_MAX. */
+int xt_pages_copy(const xt_page_buffer* buffers, int n_buffers, const int32_t* moves, int64_t moves_stride, int n,
+                  const int32_t* count, xt_stream_t stream);
+
 /* --- Top-k producers: the indexer logits and the selection of each query's keys ----------------------------- */
 
 /* Replaces qsa_prefill.qsa_mqa_prefill (xtier/packs/qwen4_exp/qsa_prefill.py:77-102, the kernel at :22-74 and the

@@ -45,8 +45,15 @@ class MlaFp8Cache(ctypes.Structure):
     _fields_ = [('pages', _P), ('num_pages', _L), ('page_size', _I), ('page_stride', _L)]
 
 
+class PageBuffer(ctypes.Structure):
+    """xt_page_buffer: the pages of one buffer (stride and size of a page in bytes)."""
+    _fields_ = [('base', _P), ('pages', _L), ('stride', _L), ('bytes', _L)]
+
+
 _CP, _KP, _FP = ctypes.POINTER(MlaCache), ctypes.POINTER(MlaKeys), ctypes.POINTER(MlaFp8Cache)
 _SP = ctypes.POINTER(KvStore)
+_BP = ctypes.POINTER(PageBuffer)
+PAGES_COPY_MAX = 64
 
 SIGNATURES = {
     'xt_version': (_I, []),
@@ -79,6 +86,17 @@ SIGNATURES = {
     'xt_sparse_mla_workspace_bytes': (_Z, [_I, _I, _I]),
     'xt_sparse_mla_fp8_workspace_bytes': (_Z, [_I, _I, _I]),
     'xt_sparse_mla_max_split_keys': (_I, [_I]),
+    'xt_page8_append': (_I, [_P, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _L, _I, _I, _I, _L, _L, _L, _L, _P, _L, _I, _P,
+                             _P, _I, _P]),
+    'xt_page8_attention_workspace_bytes': (_Z, [_I, _I, _I, _I, _I]),
+    'xt_page8_attention': (_I, [_P, _L, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _L, _L, _L, _L, _P, _L, _I, _P, _P, _I,
+                                _I, _I, _I, _F, _P, _L, _L, _I, _P, _P, _Z, _P]),
+    'xt_pages_workspace_bytes': (_Z, [_L, _I]),
+    'xt_pages_extend': (_I, [_P, _L, _P, _L, _I, _P, _P, _I, _I, _P, _P, _Z, _P]),
+    'xt_pages_fork': (_I, [_P, _L, _P, _L, _I, _P, _I, _I, _P, _P, _I, _P, _L, _P, _Z, _P]),
+    'xt_pages_free': (_I, [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P]),
+    'xt_pages_compact': (_I, [_P, _L, _P, _L, _I, _I, _P, _P, _P, _Z, _P]),
+    'xt_pages_copy': (_I, [_BP, _I, _P, _L, _I, _P, _P]),
     'xt_selftest_conversions_bytes': (_Z, []),
     'xt_selftest_conversions': (_I, [_P, _P]),
     'xt_ceiling_mfma': (_I, [_P, ctypes.c_int, ctypes.c_int, _P]),

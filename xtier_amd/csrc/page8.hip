@@ -1,0 +1,909 @@
+// The 8-bit paged cache: quantize-on-append with one power-of-two scale for each page and head, and attention over
+// such pages (decode, verification, prompt chunks; whole contexts or a sliding window with sinks). Definitions and
+// layouts in include/xtier_amd.h.
+//
+// Layout. Per page and KV head the K block is [page, dim] E4M3 bytes, and the V block is stored transposed, [dim, page].
+// With keys as rows of the first product (S^T = K Q^T) a lane of an MFMA result holds one query and several keys, which
+// is the operand shape that the second product (O^T = V^T P^T) wants for P^T, so P never leaves its registers; V^T rows
+// are then what its first operand wants, 16 bytes a lane, with no transpose anywhere in the attention. The append,
+// which touches each value once, pays for the transpose.
+//
+// Scales are powers of two. E4M3 has the same relative precision everywhere above 2^-6, so a finer scale would gain
+// less than one binade of range, while a power of two makes every step but the rounding to E4M3 exact: a page whose
+// scale grows keeps its normal values unchanged, and a K value with its scale is a BF16 value, so the first product takes
+// the BF16 query and the keys exactly.
+#include "xt_common.h"
+#include "xt_host.h"
+
+namespace xt {
+namespace {
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 64;               // keys of a step
+constexpr int kMinExp = 63, kMaxExp = 246;   // scale exponents an append writes: 2^-64 .. 2^119, so that 448 * scale is finite
+
+__device__ inline float exp_bits(int biased) {   // 2^(biased - 127), biased clamped to 1 .. 254
+  const int e = biased < 1 ? 1 : biased > 254 ? 254 : biased;
+  return __uint_as_float((uint32_t)e << 23);
+}
+
+// --- append -----------------------------------------------------------------------------------------------------------
+
+struct AppendArgs {
+  const uint16_t *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  int64_t rows;
+  uint8_t *kp, *vp, *ke, *ve;
+  int64_t page_stride, head_stride, exp_page_stride, exp_head_stride;
+  int64_t pages;
+  int page_shift, heads, dim;
+  const int32_t* table;
+  int64_t table_stride;
+  int width;
+  const int32_t *seq_lens, *cu_rows;
+  int batch;
+};
+
+// The biased exponent of the smallest power of two that keeps a BF16 magnitude (its bits) within 448 = 1.75 * 2^8.
+__device__ inline int scale_exponent(uint32_t mag) {
+  const int e = (int)(mag >> 7) - 8 + ((mag & 0x7Fu) > 0x60u ? 1 : 0);
+  return e < kMinExp ? kMinExp : e > kMaxExp ? kMaxExp : e;
+}
+
+// Two values rounded to E4M3 (nearest even); more than 448 (infinities too) becomes 448, a NaN stays one.
+__device__ inline uint32_t e4m3_pair(float a, float b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  a = __builtin_fabsf(a) > 448.0f ? __builtin_copysignf(448.0f, a) : a;
+  b = __builtin_fabsf(b) > 448.0f ? __builtin_copysignf(448.0f, b) : b;
+  uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xFFFFu;
+  // (the conversion makes every NaN 0xFF: keep its sign, as the rest of the library does)
+  if (a != a) w = (w & 0xFF00u) | 0x7Fu | (__float_as_uint(a) >> 24 & 0x80u);
+  if (b != b) w = (w & 0xFFu) | 0x7F00u | (__float_as_uint(b) >> 16 & 0x8000u);
+  return w;
+#else
+  return 0;
+#endif
+}
+
+// One workgroup per (touched page, head). The page's new rows are read twice, once for their largest magnitude and once
+// to quantize them (the second time from L2).
+template <int T>
+__global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
+  extern __shared__ uint8_t s_vt[];   // [dim][page + 4] bytes of the new V rows
+  __shared__ uint32_t s_mag[2];
+  const int head = (int)blockIdx.y;
+  const int64_t unit = blockIdx.x;
+  const int page = 1 << a.page_shift;
+  int b;
+  int64_t ordinal, row0, n;
+  if (!a.cu_rows) {
+    b = (int)unit;
+    ordinal = 0;
+    row0 = b;
+    n = 1;
+  } else {
+    // request b's units start at floor(cu[b] / page) + 2 b: n rows touch at most floor(n / page) + 2 pages
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((a.cu_rows[mid] >> a.page_shift) + 2 * (int64_t)mid <= unit) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    row0 = a.cu_rows[b];
+    n = a.cu_rows[b + 1] - row0;
+    ordinal = unit - ((row0 >> a.page_shift) + 2 * (int64_t)b);
+  }
+  const int64_t len = a.seq_lens[b];
+  const int64_t start = len - n;                              // the position of the request's first row
+  const int64_t first = start > 0 ? start : 0;
+  const int64_t col = (first >> a.page_shift) + ordinal;
+  const int64_t lo = max(first, col << a.page_shift), hi = min(len, (col + 1) << a.page_shift);
+  if (ordinal < 0 || n <= 0 || lo >= hi || col >= a.width) return;
+  const int32_t id = a.table[(int64_t)b * a.table_stride + col];
+  if (id < 0 || id >= a.pages) return;
+  const int64_t src0 = row0 + (lo - start);                   // the first row of k / v for this page
+  const int t0 = (int)(lo & (page - 1)), m = (int)(hi - lo);
+  if (src0 < 0 || src0 + m > a.rows) return;
+  if (threadIdx.x < 2) s_mag[threadIdx.x] = 0;
+  __syncthreads();
+
+  const int vecs = a.dim / 8;         // 16-byte pieces of a row
+  const uint16_t* ks = a.k + src0 * a.k_row + head * a.k_head;
+  const uint16_t* vs = a.v + src0 * a.v_row + head * a.v_head;
+  auto largest = [](uint4 w, uint32_t mag) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = ws[i] & 0x7FFFu, y = (ws[i] >> 16) & 0x7FFFu;   // magnitudes; infinities and NaN do not count
+      mag = max(mag, x < 0x7F80u ? x : 0u);
+      mag = max(mag, y < 0x7F80u ? y : 0u);
+    }
+    return mag;
+  };
+  uint32_t km = 0, vm = 0;
+  for (int i = (int)threadIdx.x; i < m * vecs; i += T) {
+    const int r = i / vecs, d = i % vecs * 8;
+    km = largest(*reinterpret_cast<const uint4*>(ks + r * a.k_row + d), km);
+    vm = largest(*reinterpret_cast<const uint4*>(vs + r * a.v_row + d), vm);
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) {
+    km = max(km, (uint32_t)__shfl_xor((int)km, s));
+    vm = max(vm, (uint32_t)__shfl_xor((int)vm, s));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    atomicMax(&s_mag[0], km);
+    atomicMax(&s_mag[1], vm);
+  }
+  uint8_t* ke = a.ke + id * a.exp_page_stride + head * a.exp_head_stride;
+  uint8_t* ve = a.ve + id * a.exp_page_stride + head * a.exp_head_stride;
+  // a page that takes its first row starts anew
+  const int ke0 = t0 > 0 ? *ke : 0, ve0 = t0 > 0 ? *ve : 0;
+  __syncthreads();
+  const int ke1 = max(ke0, scale_exponent(s_mag[0])), ve1 = max(ve0, scale_exponent(s_mag[1]));
+  const float kmul = exp_bits(254 - ke1), vmul = exp_bits(254 - ve1);   // 2^(127 - e)
+  uint8_t* kp = a.kp + id * a.page_stride + head * a.head_stride;
+  uint8_t* vp = a.vp + id * a.page_stride + head * a.head_stride;
+
+  // the page's earlier rows, where the scale grew
+  if (t0 > 0 && ke1 > ke0) {
+    const float f = exp_bits(127 - (ke1 - ke0));
+    for (int i = (int)threadIdx.x; i < t0 * a.dim; i += T) {
+      const float x = e4m3_decode(kp[i]) * f;
+      kp[i] = (uint8_t)e4m3_pair(x, x);
+    }
+  }
+  if (t0 > 0 && ve1 > ve0) {
+    const float f = exp_bits(127 - (ve1 - ve0));
+    for (int i = (int)threadIdx.x; i < t0 * a.dim; i += T) {
+      uint8_t* p = vp + (i / t0 << a.page_shift) + i % t0;
+      const float x = e4m3_decode(*p) * f;
+      *p = (uint8_t)e4m3_pair(x, x);
+    }
+  }
+  // the new rows: K as they lie, V through LDS
+  auto quantize = [](uint4 w, float mul) {
+    uint2 q;
+    q.x = e4m3_pair(bf16_bits_to_f32(w.x & 0xFFFFu) * mul, bf16_bits_to_f32(w.x >> 16) * mul) |
+          e4m3_pair(bf16_bits_to_f32(w.y & 0xFFFFu) * mul, bf16_bits_to_f32(w.y >> 16) * mul) << 16;
+    q.y = e4m3_pair(bf16_bits_to_f32(w.z & 0xFFFFu) * mul, bf16_bits_to_f32(w.z >> 16) * mul) |
+          e4m3_pair(bf16_bits_to_f32(w.w & 0xFFFFu) * mul, bf16_bits_to_f32(w.w >> 16) * mul) << 16;
+    return q;
+  };
+  const int pitch = page + 4;
+  for (int i = (int)threadIdx.x; i < m * vecs; i += T) {
+    const int r = i / vecs, d = i % vecs * 8;
+    *reinterpret_cast<uint2*>(kp + (t0 + r) * a.dim + d) =
+        quantize(*reinterpret_cast<const uint4*>(ks + r * a.k_row + d), kmul);
+    const uint2 q = quantize(*reinterpret_cast<const uint4*>(vs + r * a.v_row + d), vmul);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_vt[(d + j) * pitch + t0 + r] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+  }
+  __syncthreads();
+  if (t0 % 4 == 0 && m % 4 == 0) {
+    const int words = m / 4;
+    for (int i = (int)threadIdx.x; i < a.dim * words; i += T) {
+      const int d = i / words, t = t0 + i % words * 4;
+      *reinterpret_cast<uint32_t*>(vp + (d << a.page_shift) + t) = *reinterpret_cast<uint32_t*>(s_vt + d * pitch + t);
+    }
+  } else {
+    for (int i = (int)threadIdx.x; i < a.dim * m; i += T) {
+      const int d = i / m, t = t0 + i % m;
+      vp[(d << a.page_shift) + t] = s_vt[d * pitch + t];
+    }
+  }
+  if (threadIdx.x == 0) {
+    *ke = (uint8_t)ke1;
+    *ve = (uint8_t)ve1;
+  }
+}
+
+// --- attention: the work and its division ------------------------------------------------------------------------------
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  const uint8_t *kp, *vp, *ke, *ve;
+  int64_t page_stride, head_stride, exp_page_stride, exp_head_stride;
+  int64_t pages;
+  int page_shift, heads, group;
+  const int32_t* table;
+  int64_t table_stride;
+  int width;
+  const int32_t *seq_lens, *cu_q;
+  int batch, rows;
+  int window, sinks;
+  float scale;          // softmax scale * log2(e)
+  void* out;
+  int64_t out_row, out_head;
+  int out_bf16;
+  float* lse;           // [rows, heads * group] or NULL
+  int64_t entries;      // (request, row tile) pairs, some empty
+  int min_tiles;        // key tiles that a workgroup takes at least
+  int32_t* counters;    // one per workgroup, zero between calls
+  float* part;          // per workgroup two partials
+};
+
+// A row tile of a request: rows r = token * group + head of the group, `m_rows` of them, and its key tiles. Tile t of
+// the entry holds the keys from 64 * (t < sink_tiles ? t : t + skip).
+struct Entry {
+  int b, n;             // request and its query tokens
+  int row0;             // the request's first row of q
+  int r0, r1;           // rows of the tile within the request
+  int len, start;       // context length, the position of the first query token
+  int end;              // keys that any row may see
+  int sink_tiles, skip, tiles;
+};
+
+__device__ inline Entry entry_at(const AttnArgs& a, int64_t e, int m_rows) {
+  Entry x;
+  int64_t tile;
+  if (!a.cu_q) {
+    const int per = (a.group + m_rows - 1) / m_rows;
+    x.b = (int)(e / per);
+    tile = e - (int64_t)x.b * per;
+    x.row0 = x.b;
+    x.n = 1;
+  } else {
+    // request b's tiles start at floor(cu[b] * group / m_rows) + b, which leaves room for a ragged last one
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)a.cu_q[mid] * a.group / m_rows + mid <= e) lo = mid;
+      else hi = mid - 1;
+    }
+    x.b = lo;
+    x.row0 = a.cu_q[lo];
+    x.n = a.cu_q[lo + 1] - x.row0;
+    tile = e - ((int64_t)x.row0 * a.group / m_rows + lo);
+    if (x.row0 < 0 || x.n < 0 || x.row0 + (int64_t)x.n > a.rows) x.n = 0;
+  }
+  x.len = max(a.seq_lens[x.b], 0);
+  x.start = x.len - x.n;
+  const int64_t all = (int64_t)x.n * a.group;
+  const int64_t r0 = tile * m_rows, r1 = r0 + m_rows < all ? r0 + m_rows : all;
+  x.r0 = x.r1 = x.end = x.sink_tiles = x.skip = x.tiles = 0;
+  if (tile < 0 || r0 >= all) return x;
+  x.r0 = (int)r0;
+  x.r1 = (int)r1;
+  const int p_lo = x.start + x.r0 / a.group, p_hi = x.start + (x.r1 - 1) / a.group;
+  const int64_t cap = (int64_t)a.width << a.page_shift;
+  x.end = p_hi + 1 <= 0 ? 0 : p_hi + 1 < cap ? p_hi + 1 : (int)cap;
+  const int tiles = (int)(((int64_t)x.end + kTile - 1) / kTile);
+  if (a.window > 0) {
+    const int64_t from = (int64_t)p_lo - a.window + 1;
+    int lo = from > 0 ? (int)(from / kTile) : 0;
+    lo = lo < tiles ? lo : tiles;
+    x.sink_tiles = (int)(((int64_t)min(a.sinks, x.end) + kTile - 1) / kTile);
+    x.skip = lo > x.sink_tiles ? lo - x.sink_tiles : 0;
+  }
+  x.tiles = tiles - x.skip > 0 ? tiles - x.skip : 1;   // rows that see nothing still take a step, which writes them
+  return x;
+}
+
+// The launch divides its work, the key tiles of every (KV head, entry), into equal runs, one per workgroup, whatever
+// the lengths: a long request is shared by many workgroups and many short ones by one, and a captured launch follows the
+// lengths of each replay. Work is numbered head by head, entry by entry. A (head, entry) that several workgroups share
+// is merged from their partials by the last of them to finish, in their order.
+struct Share {
+  int64_t per, total, per_head;   // tiles of a workgroup, of the launch, of one head
+  int64_t pos, end;               // this workgroup's run
+  int head;
+  int64_t entry, entry_pos;       // the entry that holds pos, and the number of its first tile within its head
+};
+
+template <int T>
+__device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int group_id) {
+  __shared__ int64_t s_sum[T / 64];
+  __shared__ int64_t s_find[2];
+  Share sh;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t chunk = (a.entries + T - 1) / T;
+  const int64_t e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
+  int64_t sum = 0;
+  for (int64_t e = e0; e < e1; ++e) sum += entry_at(a, e, m_rows).tiles;
+  int64_t incl = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 63) s_sum[wave] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) {
+    const int64_t v = s_sum[w];
+    if (w < wave) before += v;
+    all += v;
+  }
+  sh.per_head = all;
+  sh.total = all * a.heads;
+  sh.per = (sh.total + groups - 1) / groups;
+  if (sh.per < a.min_tiles) sh.per = a.min_tiles;
+  sh.pos = sh.per * group_id;
+  sh.end = min(sh.pos + sh.per, sh.total);
+  sh.head = 0;
+  sh.entry = sh.entry_pos = 0;
+  if (sh.pos >= sh.end) return sh;
+  sh.head = (int)(sh.pos / all);
+  const int64_t want = sh.pos - sh.head * all;   // within the head
+  int64_t at = before + incl - sum;
+  if (want >= at && want < at + sum) {
+    for (int64_t e = e0; e < e1; ++e) {
+      const int t = entry_at(a, e, m_rows).tiles;
+      if (want < at + t) {
+        s_find[0] = e;
+        s_find[1] = at;
+        break;
+      }
+      at += t;
+    }
+  }
+  __syncthreads();
+  sh.entry = s_find[0];
+  sh.entry_pos = s_find[1];
+  return sh;
+}
+
+// The workgroup of the launch, renumbered so that each XCD (workgroups go round robin over 8) takes a contiguous run of
+// the work: neighbours in it read the same keys, out of that XCD's L2.
+__device__ inline int xcd_order(int id, int groups) { return (id & 7) * (groups >> 3) + (id >> 3); }
+
+__device__ inline void store_out(const AttnArgs& a, int64_t row, int head, int d, float4_t v) {
+  const int64_t at = row * a.out_row + head * a.out_head + d;
+  uint2 w;
+  if (a.out_bf16) {
+    w.x = pack2_16<true>(v[0], v[1]);
+    w.y = pack2_16<true>(v[2], v[3]);
+  } else {
+    w.x = pack2_16<false>(v[0], v[1]);
+    w.y = pack2_16<false>(v[2], v[3]);
+  }
+  *reinterpret_cast<uint2*>((uint16_t*)a.out + at) = w;
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// Eight E4M3 bytes times a power of two, as BF16 (exact: E4M3 has fewer bits, and the exponents of both fit).
+__device__ inline bf16x8_t e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ inline half8_t e4m3x8_to_f16(uint32_t lo, uint32_t hi, float scale) {
+  const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false);
+  const half2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true);
+  const half2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false);
+  const half2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
+  return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Bits 0..3 of n as byte masks.
+__device__ inline uint32_t byte_mask(uint32_t n) { return ((n & 15u) * 0x00204081u & 0x01010101u) * 0xFFu; }
+
+// The top bit of each byte that holds an E4M3 NaN (0x7F or 0xFF).
+__device__ inline uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+#endif
+
+// --- attention: few rows per request ------------------------------------------------------------------------------------
+
+// 16 * NQ query rows a workgroup; its 4 waves take the run's key tiles in turn, straight from memory into registers, and
+// merge at the end of each entry. Per tile of 64 keys a wave does S^T = K Q^T (A rows are keys, permuted so that lane
+// group g holds scores of the keys 16 g .. 16 g + 15 in the order of a V^T row), the softmax of one query column per
+// lane, and O^T += V^T P^T.
+//
+// P and V enter the second product as FP16: P is at most 1, and V as E4M3 times 2^(its page's exponent - the largest
+// exponent seen) is exact within 15 binades below the largest. BF16 would round P eight times as coarsely.
+template <int D, int NQ>
+struct DecodeGeo {
+  static constexpr int kX = D / 64;                     // 16-byte pieces of a K row per lane
+  static constexpr int kDT = D / 16;                    // 16-dim tiles of O
+  static constexpr int kRows = 16 * NQ;
+  static constexpr int kPitch = D + 4;                  // floats of a merged row in LDS: D, max, sum, padding
+  static constexpr int kLds = 4 * kRows * kPitch * 4;
+};
+
+template <int D>
+struct KvStep {
+  uint4 k[D / 64][4];       // [16-byte piece][16 keys]
+  uint4 v[D / 16];
+  int ke, ve;               // exponents of the lane's K and V blocks, -1: a block that holds nothing
+};
+
+template <int D, int NQ>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = DecodeGeo<D, NQ>;
+  constexpr int M = G::kRows;
+  extern __shared__ float s_merge[];
+  __shared__ int s_last;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int c = lane & 15, g = lane >> 4;
+  const int groups = (int)gridDim.x;
+  const int wg = xcd_order((int)blockIdx.x, groups);
+  Share sh = share_of<256>(a, M, groups, wg);
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int kk0 = 16 * (c >> 2) + (c & 3);   // A row c of 16-key tile t is key kk0 + 4 t of the 64
+
+  while (sh.pos < sh.end) {
+    // (uniform over the workgroup, and told so: the loads of an entry then go through the scalar cache)
+    const int64_t e_id = ((int64_t)__builtin_amdgcn_readfirstlane((int)(sh.entry >> 32)) << 32) |
+                         (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.entry);
+    const Entry en = entry_at(a, e_id, M);
+    const int64_t unit0 = sh.head * sh.per_head + sh.entry_pos;       // the (head, entry)'s first tile
+    const int t0 = (int)(sh.pos - unit0);
+    const int t1 = (int)min((int64_t)en.tiles, sh.end - unit0);
+    const int head = sh.head;
+
+    // query operands and positions of this lane's columns
+    bf16x8_t qb[NQ][2 * G::kX];
+    int pos[NQ];
+    int64_t q_row[NQ];
+    int q_head[NQ];
+    bool live[NQ];
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      const int r = en.r0 + 16 * nq + c;
+      live[nq] = r < en.r1;
+      // columns past the last row repeat it (with a zero query), so that they see what the others see
+      const int rr = live[nq] ? r : en.r1 - 1;
+      const int tok = rr / a.group;
+      q_row[nq] = en.row0 + tok;
+      q_head[nq] = head * a.group + (rr - tok * a.group);
+      pos[nq] = en.start + tok;
+      const uint16_t* src = a.q + q_row[nq] * a.q_row + q_head[nq] * a.q_head + 16 * g;
+#pragma unroll
+      for (int x = 0; x < G::kX; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          uint4 w = {0, 0, 0, 0};
+          if (live[nq]) w = *reinterpret_cast<const uint4*>(src + 64 * x + 8 * y);
+          qb[nq][2 * x + y] = __builtin_bit_cast(bf16x8_t, w);
+        }
+    }
+    const int p_lo = en.start + en.r0 / a.group, p_hi = en.start + (en.r1 - 1) / a.group;
+
+    float4_t acc[NQ][G::kDT];
+    float m_run[NQ], l_run[NQ];
+    int e_ref = 0;
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      m_run[nq] = -__builtin_inff();
+      l_run[nq] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < G::kDT; ++dt) acc[nq][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int32_t* row_table = a.table + (int64_t)en.b * a.table_stride;
+    auto key_of = [&](int t) { return kTile * (t < en.sink_tiles ? t : t + en.skip); };
+    auto load = [&](int t, KvStep<D>& st) {
+      const int base = key_of(t);
+      const int kblk = base + 16 * (c >> 2), vblk = base + 16 * g;
+      int kid = -1, vid = -1;
+      if (kblk < en.end) kid = row_table[kblk >> a.page_shift];
+      if (vblk < en.end) vid = row_table[vblk >> a.page_shift];
+      const bool kok = kid >= 0 && kid < a.pages, vok = vid >= 0 && vid < a.pages;
+      const int64_t ki = kok ? kid : 0, vi = vok ? vid : 0;
+      // a block that holds nothing reads page 0 and is masked
+      const uint8_t* kp = a.kp + ki * a.page_stride + head * a.head_stride + (int64_t)((base + kk0) & page_mask) * D +
+                          16 * g;
+      const uint8_t* vp = a.vp + vi * a.page_stride + head * a.head_stride + ((int64_t)c << a.page_shift) +
+                          (vblk & page_mask);
+      st.ke = a.ke[ki * a.exp_page_stride + head * a.exp_head_stride];
+      st.ve = a.ve[vi * a.exp_page_stride + head * a.exp_head_stride];
+#pragma unroll
+      for (int x = 0; x < G::kX; ++x)
+#pragma unroll
+        for (int t4 = 0; t4 < 4; ++t4)
+          st.k[x][t4] = *reinterpret_cast<const uint4*>(kp + 64 * x + 4 * t4 * D);
+#pragma unroll
+      for (int dt = 0; dt < G::kDT; ++dt)
+        st.v[dt] = *reinterpret_cast<const uint4*>(vp + ((int64_t)(16 * dt) << a.page_shift));
+      if (!kok) st.ke = -1;
+      if (!vok) st.ve = -1;
+    };
+    auto compute = [&](int t, KvStep<D>& st) {
+      const int base = key_of(t);
+      // scores
+      float4_t s[NQ][4];
+      const float ks = exp_bits(st.ke);
+#pragma unroll
+      for (int t4 = 0; t4 < 4; ++t4) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) s[nq][t4] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < G::kX; ++x) {
+          const uint4 w = st.k[x][t4];
+          const bf16x8_t k0 = e4m3x8_to_bf16(w.x, w.y, ks), k1 = e4m3x8_to_bf16(w.z, w.w, ks);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            s[nq][t4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qb[nq][2 * x], s[nq][t4], 0, 0, 0);
+            s[nq][t4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qb[nq][2 * x + 1], s[nq][t4], 0, 0, 0);
+          }
+        }
+      }
+      // a tile that every row sees whole needs no masks
+      const bool whole = base + kTile - 1 <= p_lo && base + kTile <= en.end &&
+                         (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks) &&
+                         __ballot(st.ke < 0 || st.ve < 0) == 0;
+      uint32_t vis[NQ];
+      bool slow = false;
+      int ev = st.ve;
+      // blocks of the V page that is gone hold keys that the K side masks too: lane group g's own block
+      const int j0 = base + 16 * g;
+      if (!whole) {
+        uint32_t any = 0, all = 0xFFFFu;
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+          uint32_t mask = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = j0 + i;
+            const bool see = st.ve >= 0 && j <= pos[nq] && j < en.end &&
+                             (a.window <= 0 || j > pos[nq] - a.window || j < a.sinks);
+            mask |= see ? 1u << i : 0u;
+          }
+          vis[nq] = mask;
+          any |= mask;
+          all &= mask;
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+          any |= (uint32_t)__shfl_xor((int)any, d);
+          all &= (uint32_t)__shfl_xor((int)all, d);
+        }
+        // values of keys that no row sees may be anything, NaN included: zero them. A NaN that some rows see and others
+        // do not takes the slow product below.
+        if (any == 0) ev = -1;
+        const uint32_t bm[4] = {byte_mask(any), byte_mask(any >> 4), byte_mask(any >> 8), byte_mask(any >> 12)};
+        const uint32_t some = any & ~all;
+        const uint32_t sm[4] = {byte_mask(some), byte_mask(some >> 4), byte_mask(some >> 8), byte_mask(some >> 12)};
+        uint32_t nan = 0;
+#pragma unroll
+        for (int dt = 0; dt < G::kDT; ++dt) {
+          uint4& w = st.v[dt];
+          w.x &= bm[0];
+          w.y &= bm[1];
+          w.z &= bm[2];
+          w.w &= bm[3];
+          nan |= (nan_bytes(w.x) & sm[0]) | (nan_bytes(w.y) & sm[1]) | (nan_bytes(w.z) & sm[2]) |
+                 (nan_bytes(w.w) & sm[3]);
+        }
+        slow = __ballot(nan != 0) != 0;
+      }
+      // the exponent that O is held at: the largest of any block used so far
+      const int e_new = max(e_ref, (int)max4_lanes16((float)max(ev, 0)));
+      const float e_drop = exp_bits(127 + max(e_ref - e_new, -126));
+      e_ref = e_new;
+      const float vs = exp_bits(127 + max(ev - e_ref, -126));
+      half8_t pb[NQ][2];
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq) {
+        float z[16];
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          z[i] = s[nq][i >> 2][i & 3] * a.scale;
+          if (!whole) z[i] = (vis[nq] >> i) & 1u ? z[i] : -__builtin_inff();
+          mx = max2_raw(mx, z[i]);
+        }
+        const float m_new = max2_raw(m_run[nq], max4_lanes16(mx));
+        const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run[nq] - mu);
+        m_run[nq] = m_new;
+        l_run[nq] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          z[i] = __builtin_amdgcn_exp2f(z[i] - mu);
+          l_run[nq] += z[i];
+        }
+        const float f = alpha * e_drop;
+#pragma unroll
+        for (int dt = 0; dt < G::kDT; ++dt) acc[nq][dt] *= f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pb[nq][u][i] = (_Float16)z[8 * u + i];
+      }
+      if (!slow) {
+#pragma unroll
+        for (int dt = 0; dt < G::kDT; ++dt) {
+          const uint4 w = st.v[dt];
+          const half8_t v0 = e4m3x8_to_f16(w.x, w.y, vs), v1 = e4m3x8_to_f16(w.z, w.w, vs);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pb[nq][0], acc[nq][dt], 0, 0, 0);
+            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
+          }
+        }
+      } else {
+        // NaN values are taken out of the product, and a second one of their places with each row's visible keys
+        // says which outputs they reach
+        half8_t see[NQ][2];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) see[nq][i >> 3][i & 7] = (vis[nq] >> i) & 1u ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+        for (int dt = 0; dt < G::kDT; ++dt) {
+          const uint32_t w[4] = {st.v[dt].x, st.v[dt].y, st.v[dt].z, st.v[dt].w};
+          uint32_t clean[4], bad[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t nb = nan_bytes(w[i]) >> 7;          // 1 in each NaN byte
+            clean[i] = w[i] & ~(nb * 0xFFu);
+            bad[i] = nb * 0x38u;                               // E4M3 1.0
+          }
+          const half8_t v0 = e4m3x8_to_f16(clean[0], clean[1], vs), v1 = e4m3x8_to_f16(clean[2], clean[3], vs);
+          const half8_t n0 = e4m3x8_to_f16(bad[0], bad[1], 1.0f), n1 = e4m3x8_to_f16(bad[2], bad[3], 1.0f);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pb[nq][0], acc[nq][dt], 0, 0, 0);
+            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
+            float4_t hit = float4_t{0.f, 0.f, 0.f, 0.f};
+            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(n0, see[nq][0], hit, 0, 0, 0);
+            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(n1, see[nq][1], hit, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[nq][dt][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[nq][dt][i];
+          }
+        }
+      }
+    };
+    KvStep<D> st;
+    for (int t = t0 + wave; t < t1; t += 4) {
+      load(t, st);
+      compute(t, st);
+    }
+
+    // the waves' states, normalized and at their true scale, through LDS: rows of [O, max, sum]
+    __syncthreads();
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      const float l = sum4_lanes16(l_run[nq]);
+      float* mine = s_merge + (wave * M + 16 * nq + c) * G::kPitch;
+      const float f = l != 0.0f ? exp_bits(e_ref) / l : 0.0f;   // (a NaN sum gives NaN)
+#pragma unroll
+      for (int dt = 0; dt < G::kDT; ++dt) *reinterpret_cast<float4_t*>(mine + 16 * dt + 4 * g) = acc[nq][dt] * f;
+      if (g == 0) {
+        mine[D] = m_run[nq];
+        mine[D + 1] = l;
+      }
+    }
+    __syncthreads();
+    const int64_t w_first = unit0 / sh.per, w_last = (unit0 + en.tiles - 1) / sh.per;
+    const bool alone = w_first == w_last;
+    const int rows_here = en.r1 - en.r0;
+    constexpr int kPieces = D / 4;
+    constexpr int kSlot = M * G::kPitch;                 // floats of a partial
+    const int slots = 2 * groups;
+    const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+        a.part, (short)0, (int)min((int64_t)slots * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
+    const int my_slot = 2 * wg + (sh.per * wg < unit0 ? 1 : 0);
+    // O = sum_i (w_i / sum w) O_i with w_i = 2^(m_i - max m) l_i, over the waves
+    for (int i = (int)threadIdx.x; i < rows_here * kPieces; i += 256) {
+      const int r = i / kPieces, d = i % kPieces * 4;
+      float mx = -__builtin_inff(), l = 0.0f, wt[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_merge[(w * M + r) * G::kPitch + D]);
+      const float mu = mx == -__builtin_inff() ? 0.0f : mx;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float* src = s_merge + (w * M + r) * G::kPitch;
+        wt[w] = __builtin_amdgcn_exp2f(src[D] - mu) * src[D + 1];
+        l += wt[w];
+      }
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) o += wt[w] * inv * *reinterpret_cast<float4_t*>(s_merge + (w * M + r) * G::kPitch + d);
+      if (alone) {
+        const int tok = (en.r0 + r) / a.group, qh = head * a.group + (en.r0 + r) % a.group;
+        store_out(a, en.row0 + tok, qh, d, o);
+        if (a.lse && d == 0)
+          a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] =
+              l != 0.0f ? (mx + __builtin_log2f(l)) * kLn2 : -__builtin_inff();
+      } else {
+        const int at = (my_slot * kSlot + r * G::kPitch) * 4;
+        store_partial(pr, at + 4 * d, o);
+        if (d == 0) store_partial(pr, at + 4 * D, float4_t{mx, l, 0.0f, 0.0f});
+      }
+    }
+    if (!alone) {
+      int32_t* counter = a.counters + w_first;
+      if (arrive_last(counter, (int)(w_last - w_first + 1), &s_last)) {
+        for (int i = (int)threadIdx.x; i < rows_here * kPieces; i += 256) {
+          const int r = i / kPieces, d = i % kPieces * 4;
+          float mx = -__builtin_inff(), l = 0.0f;
+          float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+          for (int64_t w = w_first; w <= w_last; ++w) {
+            const int slot = (int)(2 * w + (sh.per * w < unit0 ? 1 : 0));
+            const int at = (slot * kSlot + r * G::kPitch) * 4;
+            const float4_t ml = load_partial(pr, at + 4 * D), x = load_partial(pr, at + 4 * d);
+            // o stays normalized: both sides enter by their share of the sum
+            const float m2 = fmaxf(mx, ml[0]), mu = m2 == -__builtin_inff() ? 0.0f : m2;
+            const float w0 = l * __builtin_amdgcn_exp2f(mx - mu), w1 = ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
+            const float inv = w0 + w1 != 0.0f ? 1.0f / (w0 + w1) : 0.0f;
+            o = o * (w0 * inv) + x * (w1 * inv);
+            l = w0 + w1;
+            mx = m2;
+          }
+          const int tok = (en.r0 + r) / a.group, qh = head * a.group + (en.r0 + r) % a.group;
+          store_out(a, en.row0 + tok, qh, d, o);
+          if (a.lse && d == 0)
+            a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] =
+                l != 0.0f ? (mx + __builtin_log2f(l)) * kLn2 : -__builtin_inff();
+        }
+        reset_counter(counter);
+      }
+    }
+
+    // on to the next entry that has rows
+    sh.pos = unit0 + t1;
+    if (sh.pos < sh.end) {
+      sh.entry_pos += en.tiles;
+      do {
+        if (++sh.entry == a.entries) {
+          sh.entry = 0;
+          sh.entry_pos = 0;
+          ++sh.head;
+        }
+      } while (entry_at(a, sh.entry, M).tiles == 0);
+    }
+  }
+#endif
+}
+
+int page_shift_of(int page_size) {
+  return page_size >= 16 && page_size <= 128 && (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size)
+                                                                                    : -1;
+}
+
+// The workgroups of a launch (a multiple of 8): two to a CU.
+int attention_groups() { return 2 * device_cus() / 8 * 8; }
+
+constexpr size_t kAttnCounterBytes = 16384;   // arrival counters, one per workgroup (at most 4096)
+
+// Query rows of a decode workgroup: 32 where the requests have more than 16 on average.
+int decode_rows(int rows, int batch, int group) { return (int64_t)rows * group > 16 * (int64_t)batch ? 32 : 16; }
+
+size_t attention_workspace(int rows, int batch, int group, int dim) {
+  const int m = decode_rows(rows, batch, group);
+  return kAttnCounterBytes + (size_t)attention_groups() * 2 * m * (dim + 4) * 4;
+}
+
+}  // namespace
+}  // namespace xt
+
+using namespace xt;
+
+static int check_pool(const char* what, const void* k, const void* vt, const void* k_exp, const void* v_exp,
+                      int64_t pages, int heads, int dim, int page_size, int64_t* page_stride, int64_t* head_stride,
+                      int64_t* exp_page_stride, int64_t* exp_head_stride) {
+  if (!k || !vt || !k_exp || !v_exp) return fail(XT_EINVAL, "%s: null pool pointer", what);
+  if (dim != 64 && dim != 128 && dim != 256)
+    return fail(XT_EUNSUPPORTED, "%s: head size %d (64, 128 or 256)", what, dim);
+  if (page_shift_of(page_size) < 0)
+    return fail(XT_EUNSUPPORTED, "%s: page size %d (16, 32, 64 or 128)", what, page_size);
+  if (pages < 1 || pages > 0x7FFFFFFF || heads < 1 || heads > 65535)
+    return fail(XT_EINVAL, "%s: %lld pages, %d KV heads", what, (long long)pages, heads);
+  const int64_t block = (int64_t)page_size * dim;
+  if (*head_stride == 0) *head_stride = block;
+  if (*page_stride == 0) *page_stride = *head_stride * heads;
+  if (*exp_head_stride == 0) *exp_head_stride = 1;
+  if (*exp_page_stride == 0) *exp_page_stride = *exp_head_stride * heads;
+  if (!aligned(k, 16) || !aligned(vt, 16) || *page_stride % 16 || *head_stride % 16 || *head_stride < block ||
+      *page_stride < block || *exp_head_stride < 1 || *exp_page_stride < 1)
+    return fail(XT_EINVAL, "%s: blocks must be 16-byte aligned and %lld bytes or more apart (page stride %lld, head "
+                "stride %lld)", what, (long long)block, (long long)*page_stride, (long long)*head_stride);
+  return XT_OK;
+}
+
+static int check_rows(const char* what, const int32_t* table, int64_t table_stride, int width, const int32_t* seq_lens,
+                      const int32_t* cu, int batch, int64_t rows) {
+  if (!table || !seq_lens) return fail(XT_EINVAL, "%s: null table or lengths", what);
+  if (width < 1 || (batch > 1 && table_stride < width))
+    return fail(XT_EINVAL, "%s: table of %d columns, row stride %lld", what, width, (long long)table_stride);
+  if (!cu && rows != batch)
+    return fail(XT_EINVAL, "%s: %lld rows for %d requests without row offsets", what, (long long)rows, batch);
+  return XT_OK;
+}
+
+extern "C" int xt_page8_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                               int64_t v_row_stride, int64_t v_head_stride, int64_t rows, uint8_t* k_pages,
+                               uint8_t* vt_pages, uint8_t* k_exp, uint8_t* v_exp, int64_t pages, int kv_heads, int dim,
+                               int page_size, int64_t page_stride, int64_t head_stride, int64_t exp_page_stride,
+                               int64_t exp_head_stride, const int32_t* table, int64_t table_stride, int width,
+                               const int32_t* seq_lens, const int32_t* cu_rows, int batch, xt_stream_t stream) {
+  const char* what = "xt_page8_append";
+  if (rows < 0 || rows > 0x7FFFFFFF || batch < 0)
+    return fail(XT_EINVAL, "%s: %lld rows, %d requests", what, (long long)rows, batch);
+  if (const int st = check_pool(what, k_pages, vt_pages, k_exp, v_exp, pages, kv_heads, dim, page_size, &page_stride,
+                                &head_stride, &exp_page_stride, &exp_head_stride))
+    return st;
+  if (rows == 0 || batch == 0) return ok();
+  if (const int st = check_rows(what, table, table_stride, width, seq_lens, cu_rows, batch, rows)) return st;
+  if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || k_row_stride % 8 || v_row_stride % 8 || k_head_stride % 8 ||
+      v_head_stride % 8)
+    return fail(XT_EINVAL, "%s: k and v rows must be 16-byte aligned", what);
+  AppendArgs a{(const uint16_t*)k, (const uint16_t*)v, k_row_stride, k_head_stride, v_row_stride, v_head_stride, rows,
+               k_pages, vt_pages, k_exp, v_exp, page_stride, head_stride, exp_page_stride, exp_head_stride, pages,
+               page_shift_of(page_size), kv_heads, dim, table, table_stride, width, seq_lens, cu_rows, batch};
+  const int64_t units = cu_rows ? rows / page_size + 2 * (int64_t)batch : batch;
+  const dim3 grid((unsigned)units, kv_heads);
+  const size_t lds = (size_t)dim * (page_size + 4);
+  if (!cu_rows) append_kernel<64><<<grid, 64, lds, stream>>>(a);
+  else append_kernel<256><<<grid, 256, lds, stream>>>(a);
+  return check_launch(what);
+}
+
+extern "C" size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_heads, int kv_heads, int dim) {
+  if (rows < 0 || batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || dim < 1) return 0;
+  return attention_workspace(rows, batch, q_heads / kv_heads, dim);
+}
+
+template <int D, int NQ>
+static int launch_decode(const char* what, const AttnArgs& a, int groups, xt_stream_t stream) {
+  const size_t lds = DecodeGeo<D, NQ>::kLds;
+  if (const int st = allow_lds((const void*)decode_kernel<D, NQ>, lds, what)) return st;
+  decode_kernel<D, NQ><<<groups, 256, lds, stream>>>(a);
+  return check_launch(what);
+}
+
+extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
+                                  const uint8_t* vt_pages, const uint8_t* k_exp, const uint8_t* v_exp, int64_t pages,
+                                  int kv_heads, int q_heads, int dim, int page_size, int64_t page_stride,
+                                  int64_t head_stride, int64_t exp_page_stride, int64_t exp_head_stride,
+                                  const int32_t* table, int64_t table_stride, int width, const int32_t* seq_lens,
+                                  const int32_t* cu_q, int batch, int rows, int window, int sinks, float scale,
+                                  void* out, int64_t out_row_stride, int64_t out_head_stride, int out_dtype,
+                                  float* lse, void* workspace, size_t workspace_bytes, xt_stream_t stream) {
+  const char* what = "xt_page8_attention";
+  if (rows < 0 || batch < 0 || window < 0 || sinks < 0)
+    return fail(XT_EINVAL, "%s: negative size (%d rows, %d requests, window %d, %d sinks)", what, rows, batch, window,
+                sinks);
+  if (const int st = check_pool(what, k_pages, vt_pages, k_exp, v_exp, pages, kv_heads, dim, page_size, &page_stride,
+                                &head_stride, &exp_page_stride, &exp_head_stride))
+    return st;
+  if (q_heads < kv_heads || q_heads % kv_heads)
+    return fail(XT_EINVAL, "%s: %d query heads for %d KV heads", what, q_heads, kv_heads);
+  const int group = q_heads / kv_heads;
+  if (group > 128) return fail(XT_EUNSUPPORTED, "%s: %d query heads to a KV head, at most 128", what, group);
+  if (!(scale > 0.0f && scale < __builtin_inff()))
+    return fail(XT_EINVAL, "%s: a positive finite softmax scale expected, got %g", what, (double)scale);
+  if (out_dtype != XT_DTYPE_BF16 && out_dtype != XT_DTYPE_F16)
+    return fail(XT_EINVAL, "%s: output type %d", what, out_dtype);
+  if (rows == 0 || batch == 0) return ok();
+  if ((int64_t)rows * group > 0x7FFFFFFF / 2)
+    return fail(XT_EUNSUPPORTED, "%s: %d rows x %d heads of a group", what, rows, group);
+  if (const int st = check_rows(what, table, table_stride, width, seq_lens, cu_q, batch, rows)) return st;
+  if (!q || !out || !aligned(q, 16) || q_row_stride % 8 || q_head_stride % 8 || !aligned(out, 8) ||
+      out_row_stride % 4 || out_head_stride % 4)
+    return fail(XT_EINVAL, "%s: query rows must be 16-byte aligned, output rows 8-byte aligned", what);
+  const size_t need = attention_workspace(rows, batch, group, dim);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, workspace_bytes, need);
+  const int groups = attention_groups();
+  const int m = decode_rows(rows, batch, group);
+  AttnArgs a{(const uint16_t*)q, q_row_stride, q_head_stride, k_pages, vt_pages, k_exp, v_exp, page_stride,
+             head_stride, exp_page_stride, exp_head_stride, pages, page_shift_of(page_size), kv_heads, group, table,
+             table_stride, width, seq_lens, cu_q, batch, rows, window, sinks, scale * kLog2e, out, out_row_stride,
+             out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse,
+             cu_q ? (int64_t)rows * group / m + batch : (int64_t)batch * ((group + m - 1) / m), 4,
+             (int32_t*)workspace, (float*)((uint8_t*)workspace + kAttnCounterBytes)};
+  if (m == 16) {
+    if (dim == 64) return launch_decode<64, 1>(what, a, groups, stream);
+    if (dim == 128) return launch_decode<128, 1>(what, a, groups, stream);
+    return launch_decode<256, 1>(what, a, groups, stream);
+  }
+  if (dim == 64) return launch_decode<64, 2>(what, a, groups, stream);
+  if (dim == 128) return launch_decode<128, 2>(what, a, groups, stream);
+  return launch_decode<256, 2>(what, a, groups, stream);
+}

@@ -5,6 +5,7 @@ xtier/backend/formats.py). Tensors are torch tensors on the GPU; every call runs
 ``raw`` is the reference's tuple of a layer's pool buffers (qsa_fp4.py:43-58):
 (k_pay u8 [slots, kv_heads, dim/2], v_pay, k_scales u8 [slots, kv_heads, dim/16], v_scales, gk f32 [1], gv f32 [1]).
 """
+import contextlib
 import ctypes
 import functools
 import math
@@ -1125,3 +1126,238 @@ def minimax_prefill_scores(q, idx_pay, idx_sc, req_to_token, score, cu_seqlens, 
         ss[1], ss[2], _stream(q))
     _lib.check(status, 'minimax_prefill_scores')
     return score
+
+
+# --- the 8-bit paged cache ------------------------------------------------------------------------------------------
+
+def _one_device(what, *tensors):
+    """Every given tensor is on one GPU. Returns a context that makes it the current one."""
+    first = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError('xtier_amd: GPU tensors expected')
+        if first is None:
+            first = t.get_device()
+        elif t.get_device() != first:
+            raise ValueError(f'xtier_amd.{what}: tensors on cuda:{first} and cuda:{t.get_device()}')
+    return contextlib.nullcontext() if first == torch.cuda.current_device() else torch.cuda.device(first)
+
+
+def _int32(t):
+    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+
+
+def _check_page8(what, raw):
+    """The pool tuple of the 8-bit pages: (k [pages, heads, page, dim], vt [pages, heads, dim, page], k_exp, v_exp
+    [pages, heads]), bytes; each block contiguous, pages and heads strided alike for K and V."""
+    k, vt, k_exp, v_exp = raw
+    if k.dim() != 4 or vt.dim() != 4 or k_exp.dim() != 2:
+        raise ValueError(f'xtier_amd.{what}: blocks [pages, heads, page, dim] and scales [pages, heads] expected')
+    pages, heads, page, dim = k.shape
+    ks, vs, es = k.stride(), vt.stride(), k_exp.stride()
+    if (k.element_size() != 1 or vt.element_size() != 1 or k_exp.dtype != torch.uint8 or v_exp.dtype != torch.uint8
+            or vt.shape != (pages, heads, dim, page) or k_exp.shape != (pages, heads) or v_exp.shape != (pages, heads)
+            or ks[3] != 1 or ks[2] != dim or vs[3] != 1 or vs[2] != page or ks[:2] != vs[:2] or v_exp.stride() != es):
+        raise ValueError(f'xtier_amd.{what}: an 8-bit pool of blocks k [pages, heads, page, dim], vt [pages, heads, dim, '
+                         f'page] and scales [pages, heads] expected, got {tuple(k.shape)} {ks}, {tuple(vt.shape)} {vs}, '
+                         f'{tuple(k_exp.shape)} {es}')
+    return (k.data_ptr(), vt.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), pages, heads), dim, page, \
+        (ks[0], ks[1], es[0], es[1])
+
+
+def _page_table(what, table, seq_lens, cu, rows):
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f'xtier_amd.{what}: an int32 page table [requests, pages] with contiguous rows expected')
+    batch = table.shape[0]
+    if seq_lens.numel() != batch or (cu is not None and cu.numel() != batch + 1) or (cu is None and rows != batch):
+        raise ValueError(f'xtier_amd.{what}: {rows} rows, {seq_lens.numel()} lengths, '
+                         f'{None if cu is None else cu.numel()} row offsets for a table of {batch} requests')
+    return batch
+
+
+def page8_append(k, v, raw, table, seq_lens, cu_rows=None):
+    """Quantize-on-append into 8-bit pages: k, v BF16 [rows, kv_heads, dim] (strided rows and heads allowed), the pool's
+    ``raw`` (pool.Page8Pool.raw), its page table int32 [requests, width], seq_lens int32 [requests] with the new tokens,
+    and cu_rows int32 [requests + 1], the requests' rows (None: one row each). The n rows of a request go to its last n
+    positions. Each page and head keeps a power-of-two scale, which grows with its largest value (see
+    xt_page8_append); no page may take rows of two requests."""
+    ptrs, dim, page, strides = _check_page8('page8_append', raw)
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 3 or k.shape != v.shape \
+            or k.shape[1:] != (ptrs[5], dim) or k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError(f'xtier_amd.page8_append: BF16 rows [rows, {ptrs[5]}, {dim}] expected, got {k.dtype} '
+                         f'{tuple(k.shape)}, {v.dtype} {tuple(v.shape)}')
+    rows = k.shape[0]
+    batch = _page_table('page8_append', table, seq_lens, cu_rows, rows)
+    with _one_device('page8_append', k, v, *raw, table, seq_lens, cu_rows):
+        seq_lens, cu_rows = _int32(seq_lens), _int32(cu_rows)
+        _lib.check(_lib.lib().xt_page8_append(
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), rows, *ptrs, dim, page,
+            *strides, table.data_ptr(), table.stride(0), table.shape[1], seq_lens.data_ptr(), _ptr(cu_rows), batch,
+            _stream(k)), 'page8_append')
+
+
+_stream_workspaces = {}   # (device index, stream) -> zeroed uint8 tensor
+
+
+def _stream_workspace(t, nbytes):
+    """A zero-filled workspace for a call on t's device and its current stream: kept per stream, so calls that overlap
+    on two streams never share one; inside a graph capture a new one of the graph's own memory, so graphs never share
+    one either."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=t.device)
+    key = (t.get_device(), _stream(t))
+    buf = _stream_workspaces.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = _stream_workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=t.device)
+    return buf
+
+
+@functools.lru_cache(maxsize=1024)   # a pure function of the sizes
+def page8_workspace_bytes(rows, batch, q_heads, kv_heads, dim):
+    return int(_lib.lib().xt_page8_attention_workspace_bytes(rows, batch, q_heads, kv_heads, dim))
+
+
+def page8_attention(q, raw, table, seq_lens, scale, cu_q=None, window=0, sinks=0, out=None, lse=None, ws=None):
+    """Attention over 8-bit pages (decode, verification, prompt chunks): q BF16 [rows, q_heads, dim]; the pool's ``raw``,
+    page table, seq_lens and cu_q as page8_append takes them (the queries are each request's last tokens, their own keys
+    already appended). Each query sees the keys up to its own position, with window > 0 only the last ``window`` of them
+    and the first ``sinks``. Returns out [rows, q_heads, dim] (BF16 unless ``out`` is given, BF16 or FP16); lse FP32
+    [rows, q_heads] is filled if given. ws: a zero-filled workspace of page8_workspace_bytes, None (one per stream)."""
+    ptrs, dim, page, strides = _check_page8('page8_attention', raw)
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != dim or q.stride(2) != 1:
+        raise ValueError(f'xtier_amd.page8_attention: BF16 queries [rows, heads, {dim}] expected, got {q.dtype} '
+                         f'{tuple(q.shape)}')
+    rows, q_heads = q.shape[:2]
+    batch = _page_table('page8_attention', table, seq_lens, cu_q, rows)
+    with _one_device('page8_attention', q, *raw, table, seq_lens, cu_q, out, lse, ws):
+        if out is None:
+            out = torch.empty((rows, q_heads, dim), dtype=torch.bfloat16, device=q.device)
+        if out.dtype not in _DTYPES or out.shape != q.shape or out.stride(2) != 1:
+            raise ValueError(f'xtier_amd.page8_attention: a BF16 or FP16 output {tuple(q.shape)} with a contiguous last '
+                             f'dim expected, got {out.dtype} {tuple(out.shape)}')
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+            raise ValueError(f'xtier_amd.page8_attention: a contiguous FP32 lse {tuple(q.shape[:2])} expected')
+        if ws is None:
+            ws = _stream_workspace(q, page8_workspace_bytes(rows, batch, q_heads, ptrs[5], dim) if batch else 256)
+        seq_lens, cu_q = _int32(seq_lens), _int32(cu_q)
+        _lib.check(_lib.lib().xt_page8_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), *ptrs, q_heads, dim, page, *strides, table.data_ptr(),
+            table.stride(0), table.shape[1], seq_lens.data_ptr(), _ptr(cu_q), batch, rows, int(window), int(sinks),
+            float(scale), out.data_ptr(), out.stride(0), out.stride(1), _DTYPES[out.dtype], _ptr(lse), ws.data_ptr(),
+            ws.numel(), _stream(q)), 'page8_attention')
+    return out
+
+
+# --- pages of a cache -----------------------------------------------------------------------------------------------
+
+def _check_pages(what, refs, table, lens=None):
+    """The sizes of a page state: (pages, table row stride, width, rows)."""
+    if refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous() or table.dim() != 2 \
+            or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f'xtier_amd.{what}: int32 refs [pages] and an int32 table [rows, width] expected')
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != table.shape[:1] or not lens.is_contiguous()):
+        raise ValueError(f'xtier_amd.{what}: int32 lens [{table.shape[0]}] expected')
+    return refs.shape[0], table.stride(0), table.shape[1], table.shape[0]
+
+
+def _pages_workspace(refs, forks=0):
+    return torch.empty(refs.shape[0] + 4 * forks, dtype=torch.int32, device=refs.device)
+
+
+def pages_extend(refs, table, lens, add, page_size):
+    """Each row b of a page table grows by add[b] tokens: the lowest free pages go to the columns that it needs, in row
+    order, and lens follows. Returns granted, bool [rows]: False for a row that found too few free pages (with those
+    that the rows before it asked for) or would outgrow the table, which stays as it was. refs int32 [pages] counts the
+    table entries of each page; refs, table and lens change in place."""
+    pages, stride, width, rows = _check_pages('pages_extend', refs, table, lens)
+    if add.shape != lens.shape:
+        raise ValueError(f'xtier_amd.pages_extend: {add.numel()} sizes for {rows} rows')
+    with _one_device('pages_extend', refs, table, lens, add):
+        granted = torch.empty(rows, dtype=torch.bool, device=refs.device)
+        ws, add = _pages_workspace(refs), _int32(add)
+        _lib.check(_lib.lib().xt_pages_extend(
+            _ptr(refs), pages, _ptr(table), stride, width, _ptr(lens), _ptr(add), rows, int(page_size), _ptr(granted),
+            _ptr(ws), ws.numel() * 4, _stream(refs)), 'pages_extend')
+    return granted
+
+
+def pages_fork(refs, table, lens, parents, children, page_size):
+    """Rows children[i] become copies of rows parents[i], sharing their full pages; an unfinished last page gets a free
+    page of its own. Returns moves int32 [2, forks], the pages (from, to) that pages_copy has to copy in every layer,
+    -1 where none. A fork is skipped if its child holds tokens or is named by an earlier fork; without a free page left
+    a child gets the full pages' tokens only. refs, table and lens change in place."""
+    pages, stride, width, rows = _check_pages('pages_fork', refs, table, lens)
+    if parents.dim() != 1 or parents.shape != children.shape:
+        raise ValueError('xtier_amd.pages_fork: as many parents as children expected')
+    n = parents.shape[0]
+    with _one_device('pages_fork', refs, table, lens, parents, children):
+        moves = torch.empty((2, n), dtype=torch.int32, device=refs.device)
+        ws, parents, children = _pages_workspace(refs, n), _int32(parents), _int32(children)
+        _lib.check(_lib.lib().xt_pages_fork(
+            _ptr(refs), pages, _ptr(table), stride, width, _ptr(lens), rows, int(page_size), _ptr(parents),
+            _ptr(children), n, _ptr(moves), n, _ptr(ws), ws.numel() * 4, _stream(refs)), 'pages_fork')
+    return moves
+
+
+def pages_free(refs, table, lens, rows):
+    """Frees the table rows ``rows`` (int32 ids; one named twice is freed once): their pages lose a reference, their
+    entries become -1 and their lengths 0, in place."""
+    pages, stride, width, n_rows = _check_pages('pages_free', refs, table, lens)
+    with _one_device('pages_free', refs, table, lens, rows):
+        rows = _int32(rows)
+        _lib.check(_lib.lib().xt_pages_free(_ptr(refs), pages, _ptr(table), stride, width, _ptr(lens), n_rows,
+                                            _ptr(rows), rows.numel(), _stream(refs)), 'pages_free')
+
+
+def pages_compact(refs, table):
+    """Moves the pages in use to the front: with L of them, those at L and above go, in ascending order, to the free ones
+    below L. refs and table follow in place. Returns (moves int32 [2, pages // 2], count int32 [1]): the first count
+    columns are the pages (from, to) that pages_copy has to copy in every layer, -1 behind them."""
+    pages, stride, width, rows = _check_pages('pages_compact', refs, table)
+    with _one_device('pages_compact', refs, table):
+        moves = torch.empty((2, pages // 2), dtype=torch.int32, device=refs.device)
+        count = torch.empty(1, dtype=torch.int32, device=refs.device)
+        ws = _pages_workspace(refs)
+        _lib.check(_lib.lib().xt_pages_compact(_ptr(refs), pages, _ptr(table), stride, width, rows, _ptr(moves),
+                                               _ptr(count), _ptr(ws), ws.numel() * 4, _stream(refs)), 'pages_compact')
+    return moves, count
+
+
+class PageBuffers:
+    """The page buffers of a cache, for pages_copy: tensors [pages, ...] whose pages are contiguous (any stride between
+    them), of any type and size. A server makes one for all layers."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        descs = []
+        for t in self.tensors:
+            if t.dim() < 1 or not (t.shape[0] == 0 or t[0].is_contiguous()):
+                raise ValueError(f'xtier_amd.PageBuffers: [pages, ...] with contiguous pages expected, got '
+                                 f'{tuple(t.shape)} strides {t.stride()}')
+            size = t.element_size()
+            descs.append(_lib.PageBuffer(t.data_ptr(), t.shape[0], t.stride(0) * size,
+                                         math.prod(t.shape[1:]) * size))
+        self.guard_tensors = self.tensors[:1]
+        for t in self.tensors[1:]:
+            if t.device != self.tensors[0].device:
+                raise ValueError('xtier_amd.PageBuffers: buffers on one GPU expected')
+        most = _lib.PAGES_COPY_MAX
+        self.groups = [((_lib.PageBuffer * len(part))(*part), len(part))
+                       for part in (descs[i:i + most] for i in range(0, len(descs), most))]
+
+
+def pages_copy(buffers, moves, count=None):
+    """Copies page moves[0, i] to page moves[1, i] in every buffer (a PageBuffers, or a list of tensors [pages, ...] with
+    contiguous pages), for the columns of moves int32 [2, n] and, with count (int32 [1]), the first count of them; ids
+    outside a buffer's pages are skipped. No destination may be another move's source or destination."""
+    if not isinstance(buffers, PageBuffers):
+        buffers = PageBuffers(buffers)
+    if moves.dim() != 2 or moves.shape[0] != 2 or moves.dtype != torch.int32 \
+            or (moves.shape[1] > 1 and moves.stride(1) != 1) or (count is not None and count.dtype != torch.int32):
+        raise ValueError('xtier_amd.pages_copy: int32 moves [2, n] and an int32 count expected')
+    with _one_device('pages_copy', moves, count, *buffers.guard_tensors):
+        for descs, n in buffers.groups:
+            _lib.check(_lib.lib().xt_pages_copy(descs, n, _ptr(moves), moves.stride(0), moves.shape[1], _ptr(count),
+                                                _stream(moves)), 'pages_copy')

@@ -1,4 +1,7 @@
-"""A layer's paged NVFP4 KV pool in HBM, in either of two layouts:
+"""The caches of a layer and the pages that they live in: KVPool and LatentPool (NVFP4), Page8Pool (8 bits with a scale
+for each page and head), and PageTable, which grows, forks, frees and compacts the sequences of a server.
+
+KVPool is a layer's paged NVFP4 KV pool in HBM, in either of two layouts:
 
 - 'interleaved' (this library's layout): one uint8 buffer [slots, 2 * heads * (dim/2 + dim/16)]. Each slot holds, per
   KV head, the head's K payload row then its V payload row, and after them, per KV head, its K scales then its V
@@ -49,6 +52,13 @@ class KVPool:
     def nbytes(self):
         return sum(t.numel() for t in (self.k_pay, self.v_pay, self.k_sf, self.v_sf))
 
+    def page_buffers(self, page_size):
+        """The buffers whose pages of page_size slots move with a page of this pool (ops.PageBuffers, ops.pages_copy)."""
+        if self.slots % page_size:
+            raise ValueError(f'{self.slots} slots are not whole pages of {page_size}')
+        parts = [self.buffer] if self.buffer is not None else [self.k_pay, self.v_pay, self.k_sf, self.v_sf]
+        return [t.view(self.slots // page_size, -1) for t in parts]
+
     def set_global_scales(self, k, v):
         """The per-tensor global scales amax / (6 * 448) of K and V (formats.py:122), computed on the device."""
         ops.global_scale(k, out=self.gk)
@@ -90,6 +100,13 @@ class LatentPool:
     def raw(self):
         return (self.pay, self.scales, self.rope, self.g)
 
+    def page_buffers(self, page_size):
+        """The buffers whose pages of page_size slots move with a page of this pool (ops.PageBuffers, ops.pages_copy)."""
+        if self.slots % page_size:
+            raise ValueError(f'{self.slots} slots are not whole pages of {page_size}')
+        parts = [self.buffer] if self.buffer is not None else [self.pay, self.scales, self.rope]
+        return [t.view(self.slots // page_size, -1) for t in parts]
+
     def set_global_scale(self, latent):
         """g = amax(|latent|) / (6 * 448), computed on the device (formats.py:122)."""
         self.g = ops.global_scale(latent.reshape(latent.shape[0], 1, -1))
@@ -99,3 +116,70 @@ class LatentPool:
         launch."""
         ops.store_kv([(latent, self.g, self.pay, self.scales), (rope.to(torch.bfloat16), None, self.rope, None)], slots,
                      saturate=saturate)
+
+
+class Page8Pool:
+    """One layer's 8-bit paged KV cache: `pages` pages of page_size tokens; per page and KV head a K block [page_size,
+    dim] and a transposed V block [dim, page_size] of E4M3 bytes, side by side, and the exponent of a power-of-two scale
+    for each. `raw` is (k, vt, k_exp, v_exp) as ops.page8_append and ops.page8_attention take it. Which pages hold which
+    tokens is a PageTable's matter, one for all layers."""
+
+    def __init__(self, pages, page_size, kv_heads, dim, device='cuda'):
+        if page_size not in (16, 32, 64, 128) or dim not in (64, 128, 256):
+            raise NotImplementedError(f'pages of {page_size} tokens, head size {dim}: 16, 32, 64 or 128 and 64, 128 or '
+                                      '256 expected')
+        self.pages, self.page_size, self.kv_heads, self.dim = pages, page_size, kv_heads, dim
+        self.buffer = torch.zeros(pages, kv_heads, 2, page_size * dim, dtype=torch.uint8, device=device)
+        self.exps = torch.full((pages, kv_heads, 2), 127, dtype=torch.uint8, device=device)
+        self.k = self.buffer[:, :, 0].unflatten(2, (page_size, dim))
+        self.vt = self.buffer[:, :, 1].unflatten(2, (dim, page_size))
+        self.k_exp, self.v_exp = self.exps[..., 0], self.exps[..., 1]
+
+    @property
+    def raw(self):
+        return (self.k, self.vt, self.k_exp, self.v_exp)
+
+    def nbytes(self):
+        return self.buffer.numel() + self.exps.numel()
+
+    def page_buffers(self):
+        """The buffers whose pages move with a page of this pool (ops.PageBuffers, ops.pages_copy)."""
+        return [self.buffer, self.exps]
+
+    def append(self, k, v, table, seq_lens, cu_rows=None):
+        """Quantize-on-append of K and V rows [rows, kv_heads, dim] (BF16) at each request's last positions."""
+        ops.page8_append(k, v, self.raw, table, seq_lens, cu_rows)
+
+    def attend(self, q, table, seq_lens, scale, cu_q=None, window=0, sinks=0, out=None, lse=None, ws=None):
+        """Attention of each request's last tokens over its pages (ops.page8_attention)."""
+        return ops.page8_attention(q, self.raw, table, seq_lens, scale, cu_q, window, sinks, out, lse, ws)
+
+
+class PageTable:
+    """The pages of `rows` sequences in caches of `pages` pages, on the device: table int32 [rows, width] (-1: none), lens
+    int32 [rows] and refs int32 [pages], the table entries that name each page. Only full pages are shared (by forks),
+    so every sequence may append to its last page. The methods return what ops.pages_* return."""
+
+    def __init__(self, rows, width, pages, page_size, device='cuda'):
+        if page_size < 1 or page_size & (page_size - 1):
+            raise ValueError(f'page size {page_size}: a power of 2 expected')
+        self.page_size = page_size
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
+
+    def extend(self, add):
+        """Room for add[b] more tokens of each row b (int32 [rows]); which rows got theirs, bool [rows]."""
+        return ops.pages_extend(self.refs, self.table, self.lens, add, self.page_size)
+
+    def fork(self, parents, children):
+        """Rows `children` become copies of rows `parents`; the moves to copy in every layer."""
+        return ops.pages_fork(self.refs, self.table, self.lens, parents, children, self.page_size)
+
+    def free(self, rows):
+        """Frees rows."""
+        ops.pages_free(self.refs, self.table, self.lens, rows)
+
+    def compact(self):
+        """Moves the pages in use to the front; (moves, count) to copy in every layer."""
+        return ops.pages_compact(self.refs, self.table)
