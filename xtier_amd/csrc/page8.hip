@@ -353,6 +353,20 @@ __device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int 
 // the work: neighbours in it read the same keys, out of that XCD's L2.
 __device__ inline int xcd_order(int id, int groups) { return (id & 7) * (groups >> 3) + (id >> 3); }
 
+// On to the run's next entry that has rows, after the tiles of `sh.entry` up to t1 (unit0: its first tile).
+__device__ inline void next_entry(const AttnArgs& a, Share& sh, int64_t unit0, int t1, int tiles, int m_rows) {
+  sh.pos = unit0 + t1;
+  if (sh.pos >= sh.end) return;
+  sh.entry_pos += tiles;
+  do {
+    if (++sh.entry == a.entries) {
+      sh.entry = 0;
+      sh.entry_pos = 0;
+      ++sh.head;
+    }
+  } while (entry_at(a, sh.entry, m_rows).tiles == 0);
+}
+
 __device__ inline void store_out(const AttnArgs& a, int64_t row, int head, int d, float4_t v) {
   const int64_t at = row * a.out_row + head * a.out_head + d;
   uint2 w;
@@ -364,6 +378,19 @@ __device__ inline void store_out(const AttnArgs& a, int64_t row, int head, int d
     w.y = pack2_16<false>(v[2], v[3]);
   }
   *reinterpret_cast<uint2*>((uint16_t*)a.out + at) = w;
+}
+
+// The keys that a row at position p sees, as bounds on j - base: j < hi and (j >= lo or j < sink).
+struct Sight {
+  int hi, lo, sink;
+  __device__ bool sees(int i) const { return (i < hi) & ((i >= lo) | (i < sink)); }
+};
+__device__ inline Sight sight_of(const AttnArgs& a, int p_hi, int p_lo, int end, int base) {
+  Sight x;
+  x.hi = min(p_hi + 1, end) - base;
+  x.lo = a.window > 0 ? p_lo - a.window + 1 - base : -base;
+  x.sink = (a.window > 0 ? a.sinks : 0) - base;
+  return x;
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -390,6 +417,95 @@ __device__ inline uint32_t byte_mask(uint32_t n) { return ((n & 15u) * 0x0020408
 // The top bit of each byte that holds an E4M3 NaN (0x7F or 0xFF).
 __device__ inline uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
+// Takes the NaN values of the keys `some` (bit i: byte i) out of 16 V bytes; returns which keys held one.
+__device__ inline uint32_t take_nan(uint4& w, uint32_t some) {
+  uint32_t* const ws[4] = {&w.x, &w.y, &w.z, &w.w};
+  uint32_t found = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t nb = (nan_bytes(*ws[i]) & byte_mask(some >> (4 * i))) >> 7;   // 1 in each such byte
+    *ws[i] &= ~(nb * 0xFFu);
+    found |= (nb * 0x01020408u >> 24 & 15u) << (4 * i);                          // the four bits side by side
+  }
+  return found;
+}
+
+#endif
+
+#if defined(__HIP_DEVICE_COMPILE__)
+
+// The natural logarithm of a sum 2^m l, -inf for no keys.
+__device__ inline float lse_of(float m, float l) {
+  return l != 0.0f ? (m + __builtin_log2f(l)) * kLn2 : -__builtin_inff();
+}
+
+// The last workgroup of a (head, entry) merges its partials, slots of [rows][D O values, max, sum, padding]: normalized
+// outputs, their maximum (of scaled scores in base 2) and their sum relative to it. Reads miss every cache, so a thread
+// has those of UB pieces of CB workgroups in flight at once.
+template <int D, int M, int T, int UB, int CB>
+__device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int head, int64_t unit0, int64_t per,
+                                      int64_t w_first, int64_t w_last, __amdgpu_buffer_rsrc_t pr) {
+  constexpr int kPieces = D / 4, kPitch = D + 4, kSlot = M * kPitch;
+  const int units = (en.r1 - en.r0) * kPieces;
+  for (int i0 = (int)threadIdx.x; i0 < units; i0 += T * UB) {
+    float mx[UB], l[UB];
+    float4_t o[UB];
+#pragma unroll
+    for (int k = 0; k < UB; ++k) {
+      mx[k] = -__builtin_inff();
+      l[k] = 0.0f;
+      o[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int64_t w0 = w_first; w0 <= w_last; w0 += CB) {
+      float4_t ml[UB][CB], x[UB][CB];
+#pragma unroll
+      for (int k = 0; k < UB; ++k)
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          const int64_t w = w0 + c;
+          const int i = i0 + k * T;
+          // (past the last workgroup or piece: an offset past the buffer, which reads zeros)
+          const bool real = w <= w_last && i < units;
+          const int at = real ? ((int)(2 * w + (per * w < unit0 ? 1 : 0)) * kSlot + i / kPieces * kPitch) * 4 : -16;
+          ml[k][c] = load_partial(pr, real ? at + 4 * D : -16);
+          x[k][c] = load_partial(pr, real ? at + i % kPieces * 16 : -16);
+          if (!real) ml[k][c][0] = -__builtin_inff();
+        }
+#pragma unroll
+      for (int k = 0; k < UB; ++k) {
+        float m = mx[k];
+#pragma unroll
+        for (int c = 0; c < CB; ++c) m = fmaxf(m, ml[k][c][0]);
+        const float mu = m == -__builtin_inff() ? 0.0f : m;
+        // shares of the sum, so that o stays a convex combination
+        float wt[CB];
+        const float old = l[k] * __builtin_amdgcn_exp2f(mx[k] - mu);
+        float sum = old;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          wt[c] = ml[k][c][1] * __builtin_amdgcn_exp2f(ml[k][c][0] - mu);
+          sum += wt[c];
+        }
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        o[k] *= old * inv;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) o[k] += wt[c] * inv * x[k][c];
+        l[k] = sum;
+        mx[k] = m;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < UB; ++k) {
+      const int i = i0 + k * T;
+      if (i >= units) continue;
+      const int r = en.r0 + i / kPieces, d = i % kPieces * 4;
+      const int tok = r / a.group, qh = head * a.group + r % a.group;
+      store_out(a, en.row0 + tok, qh, d, o[k]);
+      if (a.lse && d == 0) a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] = lse_of(mx[k], l[k]);
+    }
+  }
+}
+
 #endif
 
 // --- attention: few rows per request ------------------------------------------------------------------------------------
@@ -408,6 +524,7 @@ struct DecodeGeo {
   static constexpr int kRows = 16 * NQ;
   static constexpr int kPitch = D + 4;                  // floats of a merged row in LDS: D, max, sum, padding
   static constexpr int kLds = 4 * kRows * kPitch * 4;
+  static constexpr int kPoison = D > 128 ? 2 : 1;       // words of D / 4 bits
 };
 
 template <int D>
@@ -472,7 +589,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
 
     float4_t acc[NQ][G::kDT];
     float m_run[NQ], l_run[NQ];
+    uint32_t poison[NQ][G::kPoison] = {};     // outputs that a NaN reached which not every row sees: bit 4 dt + i
     int e_ref = 0;
+    __syncthreads();                          // (the LDS of an earlier entry's merge is free)
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
       m_run[nq] = -__builtin_inff();
@@ -534,7 +653,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
                          (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks) &&
                          __ballot(st.ke < 0 || st.ve < 0) == 0;
       uint32_t vis[NQ];
-      bool slow = false;
       int ev = st.ve;
       // blocks of the V page that is gone hold keys that the K side masks too: lane group g's own block
       const int j0 = base + 16 * g;
@@ -542,14 +660,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
         uint32_t any = 0, all = 0xFFFFu;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
+          const Sight sight = sight_of(a, pos[nq], pos[nq], en.end, j0);
           uint32_t mask = 0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = j0 + i;
-            const bool see = st.ve >= 0 && j <= pos[nq] && j < en.end &&
-                             (a.window <= 0 || j > pos[nq] - a.window || j < a.sinks);
-            mask |= see ? 1u << i : 0u;
-          }
+          for (int i = 0; i < 16; ++i) mask |= sight.sees(i) ? 1u << i : 0u;
+          mask = st.ve >= 0 ? mask : 0u;
           vis[nq] = mask;
           any |= mask;
           all &= mask;
@@ -559,24 +674,45 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
           any |= (uint32_t)__shfl_xor((int)any, d);
           all &= (uint32_t)__shfl_xor((int)all, d);
         }
-        // values of keys that no row sees may be anything, NaN included: zero them. A NaN that some rows see and others
-        // do not takes the slow product below.
+        // values of keys that no row sees may be anything, NaN included: zero them
         if (any == 0) ev = -1;
-        const uint32_t bm[4] = {byte_mask(any), byte_mask(any >> 4), byte_mask(any >> 8), byte_mask(any >> 12)};
-        const uint32_t some = any & ~all;
-        const uint32_t sm[4] = {byte_mask(some), byte_mask(some >> 4), byte_mask(some >> 8), byte_mask(some >> 12)};
         uint32_t nan = 0;
 #pragma unroll
         for (int dt = 0; dt < G::kDT; ++dt) {
           uint4& w = st.v[dt];
-          w.x &= bm[0];
-          w.y &= bm[1];
-          w.z &= bm[2];
-          w.w &= bm[3];
-          nan |= (nan_bytes(w.x) & sm[0]) | (nan_bytes(w.y) & sm[1]) | (nan_bytes(w.z) & sm[2]) |
-                 (nan_bytes(w.w) & sm[3]);
+          w.x &= byte_mask(any);
+          w.y &= byte_mask(any >> 4);
+          w.z &= byte_mask(any >> 8);
+          w.w &= byte_mask(any >> 12);
+          nan |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
         }
-        slow = __ballot(nan != 0) != 0;
+        const uint32_t some = any & ~all;
+        if (__ballot((nan != 0) & (some != 0))) {
+          // a NaN that some rows see and others do not: it leaves the product, and the outputs that it reaches become
+          // NaN at the end. Which keys of a dimension hold one, and which keys a row sees, meet in LDS.
+          uint16_t* map = reinterpret_cast<uint16_t*>(s_merge + wave * M * G::kPitch);   // [dim][4 blocks of 16 keys]
+          uint16_t* seen = map + D * 4;                                                  // [row][4 blocks]
+#pragma unroll
+          for (int dt = 0; dt < G::kDT; ++dt) map[(16 * dt + c) * 4 + g] = (uint16_t)take_nan(st.v[dt], some);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) seen[(16 * nq + c) * 4 + g] = (uint16_t)vis[nq];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            const uint2 row = *reinterpret_cast<const uint2*>(seen + (16 * nq + c) * 4);
+#pragma unroll 1
+            for (int k = 0; k < D / 4; ++k) {          // acc[nq][k / 4][k % 4]: dimension 16 (k / 4) + 4 g + k % 4
+              const uint2 dim = *reinterpret_cast<const uint2*>(map + (16 * (k >> 2) + 4 * g + (k & 3)) * 4);
+              if ((dim.x & row.x) | (dim.y & row.y)) {
+                if (k < 32) poison[nq][0] |= 1u << k;
+                else poison[nq][G::kPoison - 1] |= 1u << (k - 32);
+              }
+            }
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
       }
       // the exponent that O is held at: the largest of any block used so far
       const int e_new = max(e_ref, (int)max4_lanes16((float)max(ev, 0)));
@@ -612,48 +748,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
 #pragma unroll
           for (int i = 0; i < 8; ++i) pb[nq][u][i] = (_Float16)z[8 * u + i];
       }
-      if (!slow) {
 #pragma unroll
-        for (int dt = 0; dt < G::kDT; ++dt) {
-          const uint4 w = st.v[dt];
-          const half8_t v0 = e4m3x8_to_f16(w.x, w.y, vs), v1 = e4m3x8_to_f16(w.z, w.w, vs);
+      for (int dt = 0; dt < G::kDT; ++dt) {
+        const uint4 w = st.v[dt];
+        const half8_t v0 = e4m3x8_to_f16(w.x, w.y, vs), v1 = e4m3x8_to_f16(w.z, w.w, vs);
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) {
-            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pb[nq][0], acc[nq][dt], 0, 0, 0);
-            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
-          }
-        }
-      } else {
-        // NaN values are taken out of the product, and a second one of their places with each row's visible keys
-        // says which outputs they reach
-        half8_t see[NQ][2];
-#pragma unroll
-        for (int nq = 0; nq < NQ; ++nq)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) see[nq][i >> 3][i & 7] = (vis[nq] >> i) & 1u ? (_Float16)1.0f : (_Float16)0.0f;
-#pragma unroll
-        for (int dt = 0; dt < G::kDT; ++dt) {
-          const uint32_t w[4] = {st.v[dt].x, st.v[dt].y, st.v[dt].z, st.v[dt].w};
-          uint32_t clean[4], bad[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t nb = nan_bytes(w[i]) >> 7;          // 1 in each NaN byte
-            clean[i] = w[i] & ~(nb * 0xFFu);
-            bad[i] = nb * 0x38u;                               // E4M3 1.0
-          }
-          const half8_t v0 = e4m3x8_to_f16(clean[0], clean[1], vs), v1 = e4m3x8_to_f16(clean[2], clean[3], vs);
-          const half8_t n0 = e4m3x8_to_f16(bad[0], bad[1], 1.0f), n1 = e4m3x8_to_f16(bad[2], bad[3], 1.0f);
-#pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) {
-            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pb[nq][0], acc[nq][dt], 0, 0, 0);
-            acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
-            float4_t hit = float4_t{0.f, 0.f, 0.f, 0.f};
-            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(n0, see[nq][0], hit, 0, 0, 0);
-            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(n1, see[nq][1], hit, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              acc[nq][dt][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[nq][dt][i];
-          }
+        for (int nq = 0; nq < NQ; ++nq) {
+          acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pb[nq][0], acc[nq][dt], 0, 0, 0);
+          acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
         }
       }
     };
@@ -671,7 +773,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
       float* mine = s_merge + (wave * M + 16 * nq + c) * G::kPitch;
       const float f = l != 0.0f ? exp_bits(e_ref) / l : 0.0f;   // (a NaN sum gives NaN)
 #pragma unroll
-      for (int dt = 0; dt < G::kDT; ++dt) *reinterpret_cast<float4_t*>(mine + 16 * dt + 4 * g) = acc[nq][dt] * f;
+      for (int dt = 0; dt < G::kDT; ++dt) {
+        float4_t o = acc[nq][dt] * f;
+        const uint32_t bad = poison[nq][dt / 8] >> (4 * (dt & 7));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = bad >> i & 1u ? __builtin_nanf("") : o[i];
+        *reinterpret_cast<float4_t*>(mine + 16 * dt + 4 * g) = o;
+      }
       if (g == 0) {
         mine[D] = m_run[nq];
         mine[D + 1] = l;
@@ -708,8 +816,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
         const int tok = (en.r0 + r) / a.group, qh = head * a.group + (en.r0 + r) % a.group;
         store_out(a, en.row0 + tok, qh, d, o);
         if (a.lse && d == 0)
-          a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] =
-              l != 0.0f ? (mx + __builtin_log2f(l)) * kLn2 : -__builtin_inff();
+          a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] = lse_of(mx, l);
       } else {
         const int at = (my_slot * kSlot + r * G::kPitch) * 4;
         store_partial(pr, at + 4 * d, o);
@@ -719,44 +826,326 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
     if (!alone) {
       int32_t* counter = a.counters + w_first;
       if (arrive_last(counter, (int)(w_last - w_first + 1), &s_last)) {
-        for (int i = (int)threadIdx.x; i < rows_here * kPieces; i += 256) {
-          const int r = i / kPieces, d = i % kPieces * 4;
-          float mx = -__builtin_inff(), l = 0.0f;
-          float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
-          for (int64_t w = w_first; w <= w_last; ++w) {
-            const int slot = (int)(2 * w + (sh.per * w < unit0 ? 1 : 0));
-            const int at = (slot * kSlot + r * G::kPitch) * 4;
-            const float4_t ml = load_partial(pr, at + 4 * D), x = load_partial(pr, at + 4 * d);
-            // o stays normalized: both sides enter by their share of the sum
-            const float m2 = fmaxf(mx, ml[0]), mu = m2 == -__builtin_inff() ? 0.0f : m2;
-            const float w0 = l * __builtin_amdgcn_exp2f(mx - mu), w1 = ml[1] * __builtin_amdgcn_exp2f(ml[0] - mu);
-            const float inv = w0 + w1 != 0.0f ? 1.0f / (w0 + w1) : 0.0f;
-            o = o * (w0 * inv) + x * (w1 * inv);
-            l = w0 + w1;
-            mx = m2;
-          }
-          const int tok = (en.r0 + r) / a.group, qh = head * a.group + (en.r0 + r) % a.group;
-          store_out(a, en.row0 + tok, qh, d, o);
-          if (a.lse && d == 0)
-            a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] =
-                l != 0.0f ? (mx + __builtin_log2f(l)) * kLn2 : -__builtin_inff();
-        }
+        merge_partials<D, M, 256, 1, 16>(a, en, head, unit0, sh.per, w_first, w_last, pr);
         reset_counter(counter);
       }
     }
 
-    // on to the next entry that has rows
-    sh.pos = unit0 + t1;
-    if (sh.pos < sh.end) {
-      sh.entry_pos += en.tiles;
-      do {
-        if (++sh.entry == a.entries) {
-          sh.entry = 0;
-          sh.entry_pos = 0;
-          ++sh.head;
-        }
-      } while (entry_at(a, sh.entry, M).tiles == 0);
+    next_entry(a, sh, unit0, t1, en.tiles, M);
+  }
+#endif
+}
+
+// --- attention: many rows per request -----------------------------------------------------------------------------------
+
+// 128 query rows a workgroup, 32 for each of its 4 waves, on 32x32 MFMAs. The workgroup dequantizes each 64-key tile
+// once, K to BF16 and V to FP16, into one of two LDS stages while it computes on the other: a wave's 32 rows alone would
+// pay the conversion four times over. K rows lie in LDS in the order of the A rows of S^T (key_row) and 16-byte units of
+// a row are rotated by an XOR with the row, so that the reads of 8 neighbouring lanes fall into different banks.
+template <int D>
+struct PrefillGeo {
+  static constexpr int kM = 128;
+  static constexpr int kStageK = kTile * D * 2, kStageV = D * kTile * 2;
+  static constexpr int kLds = 2 * (kStageK + kStageV);
+  static constexpr int kLoads = kTile * D / 16 / 256;    // 16-byte pieces of K, and of V, that a thread stages: D / 64
+  static constexpr int kDT = D / 32;
+};
+
+// The LDS row of a key: A row 8 a + 4 h + i of a 32-key block is key 16 (a / 2) + 8 h + 4 (a % 2) + i, which leaves
+// lane half h of S^T with eight neighbouring keys of every 16: a step's operand of P^T, in the order of a V^T row.
+__device__ inline int key_row(int key) {
+  return (key & 32) | (key & 16) | ((key >> 2 & 1) << 3) | ((key >> 3 & 1) << 2) | (key & 3);
+}
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+template <int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using G = PrefillGeo<D>;
+  constexpr int M = G::kM, kPitch = D + 4, kSlot = M * kPitch;
+  extern __shared__ uint8_t s_stage[];
+  __shared__ int s_last;
+  // whether a stage's V holds a NaN that some rows see and others do not, and where: [stage][dim][4 blocks of 16 keys]
+  __shared__ int s_nan[3];
+  __shared__ uint16_t s_where[2][D][4];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = lane & 31, hf = lane >> 5;
+  const int groups = (int)gridDim.x;
+  const int wg = xcd_order((int)blockIdx.x, groups);
+  Share sh = share_of<256>(a, M, groups, wg);
+  const int page_mask = (1 << a.page_shift) - 1;
+  if (tid < 3) s_nan[tid] = 0;
+
+  while (sh.pos < sh.end) {
+    const int64_t e_id = ((int64_t)__builtin_amdgcn_readfirstlane((int)(sh.entry >> 32)) << 32) |
+                         (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.entry);
+    const Entry en = entry_at(a, e_id, M);
+    const int64_t unit0 = sh.head * sh.per_head + sh.entry_pos;
+    const int t0 = (int)(sh.pos - unit0);
+    const int t1 = (int)min((int64_t)en.tiles, sh.end - unit0);
+    const int head = sh.head;
+
+    const int r = en.r0 + 32 * wave + c;
+    const bool live = r < en.r1;
+    const bool wave_live = en.r0 + 32 * wave < en.r1;
+    const int rr = live ? r : en.r1 - 1;
+    const int tok = rr / a.group;
+    const int64_t q_row = en.row0 + tok;
+    const int q_head = head * a.group + (rr - tok * a.group);
+    const int pos = en.start + tok;
+    bf16x8_t qb[D / 16];
+    {
+      const uint16_t* src = a.q + q_row * a.q_row + q_head * a.q_head + 8 * hf;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        uint4 w = {0, 0, 0, 0};
+        if (live) w = *reinterpret_cast<const uint4*>(src + 16 * x);
+        qb[x] = __builtin_bit_cast(bf16x8_t, w);
+      }
     }
+    const int p_lo = en.start + en.r0 / a.group, p_hi = en.start + (en.r1 - 1) / a.group;
+    const int32_t* row_table = a.table + (int64_t)en.b * a.table_stride;
+    auto key_of = [&](int t) { return kTile * (t < en.sink_tiles ? t : t + en.skip); };
+
+    // staging: thread tid holds pieces tid + 256 i of the K block (key = piece / (D / 16)) and of the V block (dimension
+    // = piece / 4, 16 keys piece % 4)
+    uint4 kw[G::kLoads], vw[G::kLoads];
+    int kexp[G::kLoads], vexp = -1;
+    const int last = max(en.end - 1, 0);            // keys past it look its page up again, and are masked
+    auto load = [&](int t) {
+      const int base = key_of(t);
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i) {
+        const int piece = tid + 256 * i, key = base + piece / (D / 16);
+        const int id = row_table[min(key, last) >> a.page_shift];
+        const int64_t page = (uint32_t)id < (uint32_t)a.pages ? id : 0;
+        kw[i] = *reinterpret_cast<const uint4*>(a.kp + page * a.page_stride + head * a.head_stride +
+                                                (int64_t)(key & page_mask) * D + piece % (D / 16) * 16);
+        kexp[i] = a.ke[page * a.exp_page_stride + head * a.exp_head_stride];
+      }
+      const int key = base + 16 * (tid & 3);       // this thread's V keys, and the block whose exponent it reads
+      const int id = row_table[min(key, last) >> a.page_shift];
+      const bool good = ((uint32_t)id < (uint32_t)a.pages) & (key < en.end);
+      const int64_t page = good ? id : 0;
+      const uint8_t* vp = a.vp + page * a.page_stride + head * a.head_stride + (key & page_mask);
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i)
+        vw[i] = *reinterpret_cast<const uint4*>(vp + ((int64_t)((tid >> 2) + 64 * i) << a.page_shift));
+      vexp = a.ve[page * a.exp_page_stride + head * a.exp_head_stride];
+      if (!good) vexp = -1;
+    };
+    int e_ref = 0;                                  // the exponent that O is held at once the staged tile is added
+    float e_drop = 1.0f;                            // and what O is multiplied by before that
+    uint32_t block_ok = 0;                          // bit b: the tile's 16-key block b has a page
+    auto whole_tile = [&](int base) {
+      return base + kTile - 1 <= p_lo && base + kTile <= en.end &&
+             (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks);
+    };
+    auto stage = [&](int t, int buf, int flag) {
+      const int base = key_of(t);
+      const uint32_t ok4 = (uint32_t)__ballot(vexp >= 0) & 15u;
+      block_ok = ok4;
+      uint8_t* sk = s_stage + buf * (G::kStageK + G::kStageV);
+      uint8_t* sv = sk + G::kStageK;
+      int ev = vexp;
+      if (!whole_tile(base) || ok4 != 15u) {
+        // values of keys that no row sees may be anything, NaN included: zero them
+        const int j0 = base + 16 * (tid & 3);
+        const Sight widest = sight_of(a, p_hi, p_lo, en.end, j0), least = sight_of(a, p_lo, p_hi, en.end, j0);
+        uint32_t any = 0, all = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          any |= widest.sees(i) ? 1u << i : 0u;
+          all |= least.sees(i) ? 1u << i : 0u;
+        }
+        if (vexp < 0) any = 0;
+        if (any == 0) ev = -1;
+        const uint32_t some = any & ~all;
+        uint32_t nan = 0;
+#pragma unroll
+        for (int i = 0; i < G::kLoads; ++i) {
+          vw[i].x &= byte_mask(any);
+          vw[i].y &= byte_mask(any >> 4);
+          vw[i].z &= byte_mask(any >> 8);
+          vw[i].w &= byte_mask(any >> 12);
+          // such a NaN leaves the product; the outputs that it reaches become NaN at the end
+          const uint32_t found = take_nan(vw[i], some);
+          s_where[buf][(tid >> 2) + 64 * i][tid & 3] = (uint16_t)found;
+          nan |= found;
+        }
+        if (nan) s_nan[flag] = 1;
+      }
+      int e_max = max(ev, 0);
+      e_max = max(e_max, __shfl_xor(e_max, 1));
+      e_max = max(e_max, __shfl_xor(e_max, 2));
+      const int e_new = max(e_ref, e_max);
+      e_drop = exp_bits(127 + max(e_ref - e_new, -126));
+      e_ref = e_new;
+      const float vs = exp_bits(127 + max(ev - e_ref, -126));
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i) {
+        const int piece = tid + 256 * i, row = key_row(piece / (D / 16)), unit = piece % (D / 16) * 2;
+        const float ks = exp_bits(kexp[i]);
+        uint8_t* dst = sk + row * D * 2;
+        *reinterpret_cast<bf16x8_t*>(dst + ((unit ^ (row & 7)) * 16)) = e4m3x8_to_bf16(kw[i].x, kw[i].y, ks);
+        *reinterpret_cast<bf16x8_t*>(dst + (((unit + 1) ^ (row & 7)) * 16)) = e4m3x8_to_bf16(kw[i].z, kw[i].w, ks);
+        const int dim = (tid >> 2) + 64 * i, vu = (tid & 3) * 2;
+        uint8_t* vdst = sv + dim * kTile * 2;
+        *reinterpret_cast<half8_t*>(vdst + ((vu ^ (dim & 7)) * 16)) = e4m3x8_to_f16(vw[i].x, vw[i].y, vs);
+        *reinterpret_cast<half8_t*>(vdst + (((vu + 1) ^ (dim & 7)) * 16)) = e4m3x8_to_f16(vw[i].z, vw[i].w, vs);
+      }
+    };
+
+    float16_t acc[G::kDT];
+    float m_run = -__builtin_inff(), l_run = 0.0f;
+    uint32_t poison[D / 64] = {};         // outputs that a NaN reached which not every row sees: bit 16 dt + 4 a + i
+#pragma unroll
+    for (int dt = 0; dt < G::kDT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+
+    __syncthreads();        // the stages' and flags' earlier readers are done
+    if (tid < 3) s_nan[tid] = 0;
+    __syncthreads();
+    load(t0);
+    stage(t0, 0, 0);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      const bool more = t + 1 < t1;
+      const float drop = e_drop;
+      const uint32_t tile_ok = block_ok;
+      if (more) load(t + 1);
+      const int slot = (t - t0) % 3;
+      if (wave_live) {
+        const int base = key_of(t);
+        const uint8_t* sk = s_stage + buf * (G::kStageK + G::kStageV);
+        const uint8_t* sv = sk + G::kStageK;
+        float16_t s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+          const uint8_t* row = sk + (32 * kb + c) * D * 2;
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+            const bf16x8_t k = *reinterpret_cast<const bf16x8_t*>(row + (((2 * x + hf) ^ (c & 7)) * 16));
+            s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qb[x], s[kb], 0, 0, 0);
+          }
+        }
+        // s[kb][4 a + i] is key base + 32 kb + 16 (a / 2) + 8 hf + 4 (a % 2) + i
+        const bool whole = whole_tile(base) && tile_ok == 15u;
+        uint32_t vis = 0xFFFFFFFFu;
+        if (!whole) {
+          vis = 0;
+          const Sight sight = sight_of(a, pos, pos, en.end, base + 8 * hf);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int in_tile = 32 * kb + 16 * (i >> 3) + (i & 7);
+              const bool see = sight.sees(in_tile) & ((tile_ok >> (in_tile >> 4) & 1u) != 0);
+              vis |= see ? 1u << (16 * kb + i) : 0u;
+              s[kb][i] = see ? s[kb][i] : -__builtin_inff();
+            }
+        }
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        {
+          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale;
+        }
+        const float m_new = fmaxf(m_run, mx);
+        const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
+        m_run = m_new;
+        half8_t pb[4];
+        float sum = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.scale, -mu));
+            sum += p;
+            pb[2 * kb + (i >> 3)][i & 7] = (_Float16)p;
+          }
+        l_run = l_run * alpha + sum;
+        const float f = alpha * drop;
+        if (__ballot(f != 1.0f)) {
+#pragma unroll
+          for (int dt = 0; dt < G::kDT; ++dt) acc[dt] *= f;
+        }
+        if (s_nan[slot]) {      // (never in a whole tile: its map is written only beside the flag)
+          // vis holds keys 16 u + 8 hf + i as bit 8 u + i: the row's 16-bit blocks are its bytes and the other half's
+          const auto sw = __builtin_amdgcn_permlane32_swap(vis, vis, false, false);
+          const uint32_t low = sw[0], high = sw[1];
+#pragma unroll 1
+          for (int k = 0; k < D / 2; ++k) {          // acc[k / 16][4 a + i]: dimension 32 (k / 16) + 8 a + 4 hf + i
+            const uint16_t* w = s_where[buf][32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hf + (k & 3)];
+            uint32_t hit = 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) hit |= w[u] & ((low >> (8 * u) & 0xFFu) | (high >> (8 * u) & 0xFFu) << 8);
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) poison[x] |= hit && k >> 5 == x ? 1u << (k & 31) : 0u;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int dt = 0; dt < G::kDT; ++dt) {
+            const half8_t v = *reinterpret_cast<const half8_t*>(sv + (32 * dt + c) * kTile * 2 +
+                                                                (((2 * u + hf) ^ (c & 7)) * 16));
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pb[u], acc[dt], 0, 0, 0);
+          }
+      }
+      if (more) stage(t + 1, buf ^ 1, (t + 1 - t0) % 3);
+      if (tid == 0) s_nan[(t + 2 - t0) % 3] = 0;      // read last in the step before this one
+      __syncthreads();
+    }
+
+    // every wave has its rows whole: outputs or partials straight from registers (acc[dt][4 a + i] is dimension
+    // 32 dt + 8 a + 4 hf + i)
+    const int64_t w_first = unit0 / sh.per, w_last = (unit0 + en.tiles - 1) / sh.per;
+    const bool alone = w_first == w_last;
+    const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+        a.part, (short)0, (int)min((int64_t)2 * groups * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
+    float l = l_run;
+    {
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+      l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    }
+    const float f = l != 0.0f ? exp_bits(e_ref) / l : 0.0f;
+    const int my_slot = 2 * wg + (sh.per * wg < unit0 ? 1 : 0);
+    if (live) {
+#pragma unroll
+      for (int dt = 0; dt < G::kDT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float4_t o = float4_t{acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]} * f;
+          const uint32_t bad = poison[dt / 2] >> (16 * (dt & 1) + 4 * q);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = bad >> i & 1u ? __builtin_nanf("") : o[i];
+          const int d = 32 * dt + 8 * q + 4 * hf;
+          if (alone) store_out(a, q_row, q_head, d, o);
+          else store_partial(pr, (my_slot * kSlot + (r - en.r0) * kPitch + d) * 4, o);
+        }
+      if (hf == 0) {
+        if (!alone) store_partial(pr, (my_slot * kSlot + (r - en.r0) * kPitch + D) * 4, float4_t{m_run, l, 0.f, 0.f});
+        else if (a.lse) a.lse[q_row * a.heads * a.group + q_head] = lse_of(m_run, l);
+      }
+    }
+    if (!alone) {
+      int32_t* counter = a.counters + w_first;
+      if (arrive_last(counter, (int)(w_last - w_first + 1), &s_last)) {
+        merge_partials<D, M, 256, 4, 4>(a, en, head, unit0, sh.per, w_first, w_last, pr);
+        reset_counter(counter);
+      }
+    }
+    next_entry(a, sh, unit0, t1, en.tiles, M);
   }
 #endif
 }
@@ -771,12 +1160,17 @@ int attention_groups() { return 2 * device_cus() / 8 * 8; }
 
 constexpr size_t kAttnCounterBytes = 16384;   // arrival counters, one per workgroup (at most 4096)
 
-// Query rows of a decode workgroup: 32 where the requests have more than 16 on average.
-int decode_rows(int rows, int batch, int group) { return (int64_t)rows * group > 16 * (int64_t)batch ? 32 : 16; }
+// Query rows of a workgroup, by the rows (tokens x heads of a group) that a request has on average: 16 or 32 in the
+// decode kernel, which reads its keys from memory wave by wave, else the prefill kernel's 128.
+int tile_rows(int rows, int batch, int group) {
+  const int64_t all = (int64_t)rows * group;
+  return all <= 16 * (int64_t)batch ? 16 : all <= 32 * (int64_t)batch ? 32 : 128;
+}
+
+constexpr int kMinTiles = 4;   // key tiles of a workgroup: one for each wave of the decode kernel
 
 size_t attention_workspace(int rows, int batch, int group, int dim) {
-  const int m = decode_rows(rows, batch, group);
-  return kAttnCounterBytes + (size_t)attention_groups() * 2 * m * (dim + 4) * 4;
+  return kAttnCounterBytes + (size_t)attention_groups() * 2 * tile_rows(rows, batch, group) * (dim + 4) * 4;
 }
 
 }  // namespace
@@ -857,6 +1251,14 @@ static int launch_decode(const char* what, const AttnArgs& a, int groups, xt_str
   return check_launch(what);
 }
 
+template <int D>
+static int launch_prefill(const char* what, const AttnArgs& a, int groups, xt_stream_t stream) {
+  const size_t lds = PrefillGeo<D>::kLds;
+  if (const int st = allow_lds((const void*)prefill_kernel<D>, lds, what)) return st;
+  prefill_kernel<D><<<groups, 256, lds, stream>>>(a);
+  return check_launch(what);
+}
+
 extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
                                   const uint8_t* vt_pages, const uint8_t* k_exp, const uint8_t* v_exp, int64_t pages,
                                   int kv_heads, int q_heads, int dim, int page_size, int64_t page_stride,
@@ -890,20 +1292,28 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
   const size_t need = attention_workspace(rows, batch, group, dim);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, workspace_bytes, need);
-  const int groups = attention_groups();
-  const int m = decode_rows(rows, batch, group);
+  const int m = tile_rows(rows, batch, group);
+  const int64_t entries = cu_q ? (int64_t)rows * group / m + batch : (int64_t)batch * ((group + m - 1) / m);
+  // no more workgroups than the table's width could keep busy
+  const int64_t most = entries * kv_heads * ((((int64_t)width * page_size + kTile - 1) / kTile + kMinTiles - 1) / kMinTiles);
+  int groups = attention_groups();
+  if (most < groups) groups = (int)((most + 7) / 8 * 8);
   AttnArgs a{(const uint16_t*)q, q_row_stride, q_head_stride, k_pages, vt_pages, k_exp, v_exp, page_stride,
              head_stride, exp_page_stride, exp_head_stride, pages, page_shift_of(page_size), kv_heads, group, table,
              table_stride, width, seq_lens, cu_q, batch, rows, window, sinks, scale * kLog2e, out, out_row_stride,
-             out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse,
-             cu_q ? (int64_t)rows * group / m + batch : (int64_t)batch * ((group + m - 1) / m), 4,
+             out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse, entries, kMinTiles,
              (int32_t*)workspace, (float*)((uint8_t*)workspace + kAttnCounterBytes)};
   if (m == 16) {
     if (dim == 64) return launch_decode<64, 1>(what, a, groups, stream);
     if (dim == 128) return launch_decode<128, 1>(what, a, groups, stream);
     return launch_decode<256, 1>(what, a, groups, stream);
   }
-  if (dim == 64) return launch_decode<64, 2>(what, a, groups, stream);
-  if (dim == 128) return launch_decode<128, 2>(what, a, groups, stream);
-  return launch_decode<256, 2>(what, a, groups, stream);
+  if (m == 32) {
+    if (dim == 64) return launch_decode<64, 2>(what, a, groups, stream);
+    if (dim == 128) return launch_decode<128, 2>(what, a, groups, stream);
+    return launch_decode<256, 2>(what, a, groups, stream);
+  }
+  if (dim == 64) return launch_prefill<64>(what, a, groups, stream);
+  if (dim == 128) return launch_prefill<128>(what, a, groups, stream);
+  return launch_prefill<256>(what, a, groups, stream);
 }
