@@ -71,7 +71,7 @@ __device__ inline uint32_t e4m3_pair(float a, float b) {
 // to quantize them (the second time from L2).
 template <int T>
 __global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
-  extern __shared__ uint8_t s_vt[];   // [dim][page + 4] bytes of the new V rows
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_vt[];   // [dim][page + 4] bytes of the new V rows
   __shared__ uint32_t s_mag[2];
   const int head = (int)blockIdx.y;
   const int64_t unit = blockIdx.x;
@@ -207,8 +207,9 @@ struct AttnArgs {
   const uint16_t* q;
   int64_t q_row, q_head;
   const uint8_t *kp, *vp, *ke, *ve;
-  int64_t page_stride, head_stride, exp_page_stride, exp_head_stride;
-  int64_t pages;
+  uint32_t page_stride, exp_page_stride;
+  int64_t head_stride, exp_head_stride;
+  uint32_t pages;
   int page_shift, heads, group;
   const int32_t* table;
   int64_t table_stride;
@@ -221,10 +222,12 @@ struct AttnArgs {
   int64_t out_row, out_head;
   int out_bf16;
   float* lse;           // [rows, heads * group] or NULL
-  int64_t entries;      // (request, row tile) pairs, some empty
+  int entries;          // (request, row tile) pairs, some empty
   int min_tiles;        // key tiles that a workgroup takes at least
-  int32_t* counters;    // one per workgroup, zero between calls
-  float* part;          // per workgroup two partials
+  int slots;            // workgroups on the CUs at once
+  int32_t* counters;    // one per partial, zero between calls
+  float* part;
+  int partials;         // what `part` has room for
 };
 
 // A row tile of a request: rows r = token * group + head of the group, `m_rows` of them, and its key tiles. Tile t of
@@ -238,13 +241,16 @@ struct Entry {
   int sink_tiles, skip, tiles;
 };
 
-__device__ inline Entry entry_at(const AttnArgs& a, int64_t e, int m_rows) {
+// The row tiles of the requests before one whose first row is `row`, some of them empty.
+__device__ inline int tile_base(const AttnArgs& a, int row, int m_rows) { return row * a.group / m_rows; }
+
+__device__ inline Entry entry_at(const AttnArgs& a, int e, int m_rows) {
   Entry x;
-  int64_t tile;
+  int tile;
   if (!a.cu_q) {
     const int per = (a.group + m_rows - 1) / m_rows;
-    x.b = (int)(e / per);
-    tile = e - (int64_t)x.b * per;
+    x.b = per == 1 ? e : e / per;
+    tile = e - x.b * per;
     x.row0 = x.b;
     x.n = 1;
   } else {
@@ -252,24 +258,25 @@ __device__ inline Entry entry_at(const AttnArgs& a, int64_t e, int m_rows) {
     int lo = 0, hi = a.batch - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)a.cu_q[mid] * a.group / m_rows + mid <= e) lo = mid;
+      if (tile_base(a, a.cu_q[mid], m_rows) + mid <= e) lo = mid;
       else hi = mid - 1;
     }
     x.b = lo;
     x.row0 = a.cu_q[lo];
     x.n = a.cu_q[lo + 1] - x.row0;
-    tile = e - ((int64_t)x.row0 * a.group / m_rows + lo);
+    tile = e - (tile_base(a, x.row0, m_rows) + lo);
     if (x.row0 < 0 || x.n < 0 || x.row0 + (int64_t)x.n > a.rows) x.n = 0;
   }
   x.len = max(a.seq_lens[x.b], 0);
   x.start = x.len - x.n;
-  const int64_t all = (int64_t)x.n * a.group;
-  const int64_t r0 = tile * m_rows, r1 = r0 + m_rows < all ? r0 + m_rows : all;
+  const int all = x.n * a.group;          // (the host keeps rows * group within 2^30)
   x.r0 = x.r1 = x.end = x.sink_tiles = x.skip = x.tiles = 0;
-  if (tile < 0 || r0 >= all) return x;
-  x.r0 = (int)r0;
-  x.r1 = (int)r1;
-  const int p_lo = x.start + x.r0 / a.group, p_hi = x.start + (x.r1 - 1) / a.group;
+  if (tile < 0 || tile > all / m_rows || tile * m_rows >= all) return x;
+  x.r0 = tile * m_rows;
+  x.r1 = min(x.r0 + m_rows, all);
+  // (one token's heads share its position)
+  const int p_lo = x.start + (x.n == 1 ? 0 : x.r0 / a.group);
+  const int p_hi = x.start + (x.n == 1 ? 0 : (x.r1 - 1) / a.group);
   const int64_t cap = (int64_t)a.width << a.page_shift;
   x.end = p_hi + 1 <= 0 ? 0 : p_hi + 1 < cap ? p_hi + 1 : (int)cap;
   const int tiles = (int)(((int64_t)x.end + kTile - 1) / kTile);
@@ -284,56 +291,149 @@ __device__ inline Entry entry_at(const AttnArgs& a, int64_t e, int m_rows) {
   return x;
 }
 
-// The launch divides its work, the key tiles of every (KV head, entry), into equal runs, one per workgroup, whatever
-// the lengths: a long request is shared by many workgroups and many short ones by one, and a captured launch follows the
-// lengths of each replay. Work is numbered head by head, entry by entry. A (head, entry) that several workgroups share
-// is merged from their partials by the last of them to finish, in their order.
+// Both kernels divide their work, the key tiles of every (KV head, entry), on the device: a long request is shared by
+// many workgroups, whatever the lengths, and a captured launch follows the lengths of each replay. Work is numbered head
+// by head, entry by entry. A (head, entry) that several workgroups share is merged from their partials by the last of
+// them to finish, in their order.
+//
+// Sums of x and y over the workgroup's threads before this one, and over all of them. `s` holds 2 * T / 64 values.
+template <int T>
+__device__ inline void block_sums(int x, int y, int* s, int* x_before, int* x_all, int* y_before, int* y_all) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  int xi = x, yi = y;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(xi, d), v = __shfl_up(yi, d);
+    if (lane >= d) {
+      xi += u;
+      yi += v;
+    }
+  }
+  __syncthreads();
+  if (lane == 63) {
+    s[wave] = xi;
+    s[T / 64 + wave] = yi;
+  }
+  __syncthreads();
+  int xb = 0, yb = 0, xs = 0, ys = 0;
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) {
+    if (w < wave) {
+      xb += s[w];
+      yb += s[T / 64 + w];
+    }
+    xs += s[w];
+    ys += s[T / 64 + w];
+  }
+  *x_before = xb + xi - x;
+  *y_before = yb + yi - y;
+  *x_all = xs;
+  *y_all = ys;
+}
+
+// A workgroup's work in the decode kernel: piece `at` of the `count` that one (head, entry) is cut into. The pieces are
+// as small as leaves all of them on the CUs at once (or, with more (head, entry) pairs than half the slots, only those
+// well above the mean are cut: a piece has at most total / (slots / 2) tiles). Cutting at pairs only keeps every
+// workgroup at one entry: equal runs that cross from one to the next cost a second entry's loads and merges in a row,
+// 8 us (measured: 1 request, 2 KV heads x 256, 4099 keys, 25 us).
+struct Piece {
+  int head, entry, at, count;
+  int slot;              // of the piece's partial, if count > 1; the slots of an entry's pieces are neighbours
+};
+
+template <int T>
+__device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
+  __shared__ int s_sum[2 * (T / 64)];
+  __shared__ int s_find[4];
+  const int tid = (int)threadIdx.x;
+  const int chunk = (a.entries + T - 1) / T;
+  const int e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
+  int sum = 0, live = 0, tiles = 0, before, all, cut_before, n_live;
+  for (int e = e0; e < e1; ++e) {
+    tiles = entry_at(a, e, m_rows).tiles;
+    sum += tiles;
+    live += tiles > 0;
+  }
+  auto tiles_of = [&](int e) { return chunk == 1 ? tiles : entry_at(a, e, m_rows).tiles; };
+  block_sums<T>(sum, live, s_sum, &before, &all, &cut_before, &n_live);
+  // per head: the smallest size that could fit, and if it does not, one that is sure to
+  const int room = max(a.slots / a.heads, 1), sure = max(max(room - n_live, room / 2), 1);
+  int size = max((all + room - 1) / room, a.min_tiles), mine, cut, per_head, cut_per_head;
+  for (int tries = 0;; ++tries) {
+    mine = cut = 0;
+    for (int e = e0; e < e1; ++e) {
+      const int n = (tiles_of(e) + size - 1) / size;
+      mine += n;
+      cut += n > 1 ? n : 0;
+    }
+    block_sums<T>(mine, cut, s_sum, &before, &per_head, &cut_before, &cut_per_head);
+    if (per_head <= room || tries == 1) break;
+    size = max((all + sure - 1) / sure, a.min_tiles);
+  }
+  Piece x;
+  x.count = 0;
+  // each XCD (workgroups go round robin over 8) takes an eighth of the pieces, neighbours in the same keys together; the
+  // grid has room for more pieces than there are, so the eighths are of what there is
+  const int of_xcd = (per_head * a.heads + 7) / 8, w = (id & 7) * of_xcd + (id >> 3);
+  if ((id >> 3) >= of_xcd || w >= per_head * a.heads) return x;
+  x.head = w / per_head;
+  int want = w - x.head * per_head - before;        // the piece, counted from this thread's first
+  if (want >= 0 && want < mine) {
+    for (int e = e0; e < e1; ++e) {
+      const int n = (tiles_of(e) + size - 1) / size;
+      if (want < n) {
+        s_find[0] = e;
+        s_find[1] = want;
+        s_find[2] = n;
+        s_find[3] = cut_before + want;
+        break;
+      }
+      want -= n;
+      cut_before += n > 1 ? n : 0;
+    }
+  }
+  __syncthreads();
+  x.entry = __builtin_amdgcn_readfirstlane(s_find[0]);
+  x.at = __builtin_amdgcn_readfirstlane(s_find[1]);
+  x.count = __builtin_amdgcn_readfirstlane(s_find[2]);
+  x.head = __builtin_amdgcn_readfirstlane(x.head);
+  x.slot = x.head * cut_per_head + __builtin_amdgcn_readfirstlane(s_find[3]);
+  return x;
+}
+
+// A workgroup's work in the prefill kernel: tiles pos .. end - 1 of the launch, equal runs for all workgroups, one per
+// slot. They are bound by their arithmetic, so equal runs end together where whole units would leave slots idle.
 struct Share {
-  int64_t per, total, per_head;   // tiles of a workgroup, of the launch, of one head
-  int64_t pos, end;               // this workgroup's run
+  int per, per_head;              // tiles of a workgroup, of one head
+  int64_t total, pos, end;        // tiles of the launch; this workgroup's run
   int head;
-  int64_t entry, entry_pos;       // the entry that holds pos, and the number of its first tile within its head
+  int entry, entry_pos;           // the entry that holds pos, and the number of its first tile within its head
 };
 
 template <int T>
 __device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int group_id) {
-  __shared__ int64_t s_sum[T / 64];
-  __shared__ int64_t s_find[2];
+  __shared__ int s_sum[2 * (T / 64)];
+  __shared__ int s_find[2];
   Share sh;
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t chunk = (a.entries + T - 1) / T;
-  const int64_t e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
-  int64_t sum = 0;
-  for (int64_t e = e0; e < e1; ++e) sum += entry_at(a, e, m_rows).tiles;
-  int64_t incl = sum;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(incl, d);
-    if (lane >= d) incl += y;
-  }
-  if (lane == 63) s_sum[wave] = incl;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < T / 64; ++w) {
-    const int64_t v = s_sum[w];
-    if (w < wave) before += v;
-    all += v;
-  }
+  const int tid = (int)threadIdx.x;
+  const int chunk = (a.entries + T - 1) / T;
+  const int e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
+  int sum = 0, before, all, unused, none;
+  for (int e = e0; e < e1; ++e) sum += entry_at(a, e, m_rows).tiles;
+  block_sums<T>(sum, 0, s_sum, &before, &all, &unused, &none);
   sh.per_head = all;
-  sh.total = all * a.heads;
-  sh.per = (sh.total + groups - 1) / groups;
+  sh.total = (int64_t)all * a.heads;
+  sh.per = (int)((sh.total + groups - 1) / groups);
   if (sh.per < a.min_tiles) sh.per = a.min_tiles;
-  sh.pos = sh.per * group_id;
+  sh.pos = (int64_t)sh.per * group_id;
   sh.end = min(sh.pos + sh.per, sh.total);
-  sh.head = 0;
-  sh.entry = sh.entry_pos = 0;
+  sh.head = sh.entry = sh.entry_pos = 0;
   if (sh.pos >= sh.end) return sh;
   sh.head = (int)(sh.pos / all);
-  const int64_t want = sh.pos - sh.head * all;   // within the head
-  int64_t at = before + incl - sum;
-  if (want >= at && want < at + sum) {
-    for (int64_t e = e0; e < e1; ++e) {
+  const int want = (int)(sh.pos - (int64_t)sh.head * all);   // within the head
+  if (want >= before && want < before + sum) {
+    int at = before;
+    for (int e = e0; e < e1; ++e) {
       const int t = entry_at(a, e, m_rows).tiles;
       if (want < at + t) {
         s_find[0] = e;
@@ -440,11 +540,11 @@ __device__ inline float lse_of(float m, float l) {
 }
 
 // The last workgroup of a (head, entry) merges its partials, slots of [rows][D O values, max, sum, padding]: normalized
-// outputs, their maximum (of scaled scores in base 2) and their sum relative to it. Reads miss every cache, so a thread
-// has those of UB pieces of CB workgroups in flight at once.
-template <int D, int M, int T, int UB, int CB>
-__device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int head, int64_t unit0, int64_t per,
-                                      int64_t w_first, int64_t w_last, __amdgpu_buffer_rsrc_t pr) {
+// outputs, their maximum (of scaled scores in base 2) and their sum relative to it. slot_of(w): workgroup w's slot.
+// Reads miss every cache, so a thread has those of UB pieces of CB workgroups in flight at once.
+template <int D, int M, int T, int UB, int CB, typename SlotOf>
+__device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int head, SlotOf slot_of,
+                                      int w_first, int w_last, __amdgpu_buffer_rsrc_t pr) {
   constexpr int kPieces = D / 4, kPitch = D + 4, kSlot = M * kPitch;
   const int units = (en.r1 - en.r0) * kPieces;
   for (int i0 = (int)threadIdx.x; i0 < units; i0 += T * UB) {
@@ -456,17 +556,17 @@ __device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int he
       l[k] = 0.0f;
       o[k] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    for (int64_t w0 = w_first; w0 <= w_last; w0 += CB) {
+    for (int w0 = w_first; w0 <= w_last; w0 += CB) {
       float4_t ml[UB][CB], x[UB][CB];
 #pragma unroll
       for (int k = 0; k < UB; ++k)
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
-          const int64_t w = w0 + c;
+          const int w = w0 + c;
           const int i = i0 + k * T;
           // (past the last workgroup or piece: an offset past the buffer, which reads zeros)
           const bool real = w <= w_last && i < units;
-          const int at = real ? ((int)(2 * w + (per * w < unit0 ? 1 : 0)) * kSlot + i / kPieces * kPitch) * 4 : -16;
+          const int at = real ? (slot_of(w) * kSlot + i / kPieces * kPitch) * 4 : -16;
           ml[k][c] = load_partial(pr, real ? at + 4 * D : -16);
           x[k][c] = load_partial(pr, real ? at + i % kPieces * 16 : -16);
           if (!real) ml[k][c][0] = -__builtin_inff();
@@ -527,11 +627,17 @@ struct DecodeGeo {
   static constexpr int kPoison = D > 128 ? 2 : 1;       // words of D / 4 bits
 };
 
+// A lane's share of a 64-key tile: the pages of its K and V blocks, then their data. What a load returns is looked at
+// where it is needed and not before: a select on it would wait for every load in flight.
+struct KvPages {
+  int k, v;
+};
 template <int D>
 struct KvStep {
   uint4 k[D / 64][4];       // [16-byte piece][16 keys]
   uint4 v[D / 16];
-  int ke, ve;               // exponents of the lane's K and V blocks, -1: a block that holds nothing
+  int ke, ve;               // scale exponents
+  bool kok, vok;            // whether the blocks hold anything
 };
 
 template <int D, int NQ>
@@ -539,26 +645,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = DecodeGeo<D, NQ>;
   constexpr int M = G::kRows;
-  extern __shared__ float s_merge[];
+  extern __shared__ __attribute__((aligned(16))) float s_merge[];
   __shared__ int s_last;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  const int groups = (int)gridDim.x;
-  const int wg = xcd_order((int)blockIdx.x, groups);
-  Share sh = share_of<256>(a, M, groups, wg);
+  const Piece pc = piece_of<256>(a, M, (int)blockIdx.x);
+  if (pc.count == 0) return;
   const int page_mask = (1 << a.page_shift) - 1;
   const int kk0 = 16 * (c >> 2) + (c & 3);   // A row c of 16-key tile t is key kk0 + 4 t of the 64
-
-  while (sh.pos < sh.end) {
-    // (uniform over the workgroup, and told so: the loads of an entry then go through the scalar cache)
-    const int64_t e_id = ((int64_t)__builtin_amdgcn_readfirstlane((int)(sh.entry >> 32)) << 32) |
-                         (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.entry);
-    const Entry en = entry_at(a, e_id, M);
-    const int64_t unit0 = sh.head * sh.per_head + sh.entry_pos;       // the (head, entry)'s first tile
-    const int t0 = (int)(sh.pos - unit0);
-    const int t1 = (int)min((int64_t)en.tiles, sh.end - unit0);
-    const int head = sh.head;
-
+  const Entry en = entry_at(a, pc.entry, M);
+  const int head = pc.head;
+  const int share = en.tiles / pc.count, longer = en.tiles % pc.count;    // the first `longer` pieces have a tile more
+  const int t0 = pc.at * share + min(pc.at, longer), t1 = t0 + share + (pc.at < longer ? 1 : 0);
+  {
     // query operands and positions of this lane's columns
     bf16x8_t qb[NQ][2 * G::kX];
     int pos[NQ];
@@ -591,7 +690,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
     float m_run[NQ], l_run[NQ];
     uint32_t poison[NQ][G::kPoison] = {};     // outputs that a NaN reached which not every row sees: bit 4 dt + i
     int e_ref = 0;
-    __syncthreads();                          // (the LDS of an earlier entry's merge is free)
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
       m_run[nq] = -__builtin_inff();
@@ -601,35 +699,50 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
     }
 
     const int32_t* row_table = a.table + (int64_t)en.b * a.table_stride;
+    const uint8_t *k_base = a.kp + head * a.head_stride, *v_base = a.vp + head * a.head_stride;
+    const uint8_t *k_exps = a.ke + head * a.exp_head_stride, *v_exps = a.ve + head * a.exp_head_stride;
     auto key_of = [&](int t) { return kTile * (t < en.sink_tiles ? t : t + en.skip); };
-    auto load = [&](int t, KvStep<D>& st) {
-      const int base = key_of(t);
-      const int kblk = base + 16 * (c >> 2), vblk = base + 16 * g;
-      int kid = -1, vid = -1;
-      if (kblk < en.end) kid = row_table[kblk >> a.page_shift];
-      if (vblk < en.end) vid = row_table[vblk >> a.page_shift];
-      const bool kok = kid >= 0 && kid < a.pages, vok = vid >= 0 && vid < a.pages;
-      const int64_t ki = kok ? kid : 0, vi = vok ? vid : 0;
-      // a block that holds nothing reads page 0 and is masked
-      const uint8_t* kp = a.kp + ki * a.page_stride + head * a.head_stride + (int64_t)((base + kk0) & page_mask) * D +
-                          16 * g;
-      const uint8_t* vp = a.vp + vi * a.page_stride + head * a.head_stride + ((int64_t)c << a.page_shift) +
-                          (vblk & page_mask);
-      st.ke = a.ke[ki * a.exp_page_stride + head * a.exp_head_stride];
-      st.ve = a.ve[vi * a.exp_page_stride + head * a.exp_head_stride];
+    const int last = max(en.end - 1, 0);       // blocks past it look its page up and are masked
+    auto pages_at = [&](int t) {
+      const int base = key_of(t), kblk = base + 16 * (c >> 2), vblk = base + 16 * g;
+      return KvPages{row_table[min(kblk, last) >> a.page_shift], row_table[min(vblk, last) >> a.page_shift]};
+    };
+    // a block that holds nothing reads page 0 and is masked
+    auto load_k = [&](int t, KvPages p, KvStep<D>& st) {
+      st.kok = ((uint32_t)p.k < a.pages) & (key_of(t) + 16 * (c >> 2) < en.end);
+      const uint32_t page = st.kok ? p.k : 0;
+      st.ke = k_exps[(uint64_t)page * a.exp_page_stride];
+      const uint8_t* kp = k_base + (uint64_t)page * a.page_stride + (((key_of(t) + kk0) & page_mask) * D + 16 * g);
 #pragma unroll
       for (int x = 0; x < G::kX; ++x)
 #pragma unroll
         for (int t4 = 0; t4 < 4; ++t4)
           st.k[x][t4] = *reinterpret_cast<const uint4*>(kp + 64 * x + 4 * t4 * D);
+    };
+    auto load_v = [&](int t, KvPages p, KvStep<D>& st) {
+      st.vok = ((uint32_t)p.v < a.pages) & (key_of(t) + 16 * g < en.end);
+      const uint32_t page = st.vok ? p.v : 0;
+      st.ve = v_exps[(uint64_t)page * a.exp_page_stride];
+      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride + ((c << a.page_shift) +
+                                                                     ((key_of(t) + 16 * g) & page_mask));
 #pragma unroll
       for (int dt = 0; dt < G::kDT; ++dt)
-        st.v[dt] = *reinterpret_cast<const uint4*>(vp + ((int64_t)(16 * dt) << a.page_shift));
-      if (!kok) st.ke = -1;
-      if (!vok) st.ve = -1;
+        st.v[dt] = *reinterpret_cast<const uint4*>(vp + ((16 * dt) << a.page_shift));
     };
-    auto compute = [&](int t, KvStep<D>& st) {
+    KvStep<D> st;
+    KvPages cur = {-1, -1}, next = {-1, -1};
+    const int first = t0 + wave;
+    if (first < t1) {
+      cur = pages_at(first);
+      if (first + 4 < t1) next = pages_at(first + 4);
+      load_k(first, cur, st);
+      load_v(first, cur, st);
+    }
+    // Each of the tile's registers is refilled as soon as its product has read it: the next K is on its way during
+    // softmax and PV, the next V during the next scores, and the pages of the tile after that.
+    for (int t = first; t < t1; t += 4) {
       const int base = key_of(t);
+      const bool more = t + 4 < t1;
       // scores
       float4_t s[NQ][4];
       const float ks = exp_bits(st.ke);
@@ -648,10 +761,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
           }
         }
       }
+      const bool pages_ok = st.kok && st.vok;
+      if (more) load_k(t + 4, next, st);
       // a tile that every row sees whole needs no masks
       const bool whole = base + kTile - 1 <= p_lo && base + kTile <= en.end &&
                          (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks) &&
-                         __ballot(st.ke < 0 || st.ve < 0) == 0;
+                         __ballot(!pages_ok) == 0;
       uint32_t vis[NQ];
       int ev = st.ve;
       // blocks of the V page that is gone hold keys that the K side masks too: lane group g's own block
@@ -664,7 +779,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
           uint32_t mask = 0;
 #pragma unroll
           for (int i = 0; i < 16; ++i) mask |= sight.sees(i) ? 1u << i : 0u;
-          mask = st.ve >= 0 ? mask : 0u;
+          mask = st.vok ? mask : 0u;
           vis[nq] = mask;
           any |= mask;
           all &= mask;
@@ -758,11 +873,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
           acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
         }
       }
-    };
-    KvStep<D> st;
-    for (int t = t0 + wave; t < t1; t += 4) {
-      load(t, st);
-      compute(t, st);
+      if (more) {
+        load_v(t + 4, next, st);
+        if (t + 8 < t1) next = pages_at(t + 8);
+      }
     }
 
     // the waves' states, normalized and at their true scale, through LDS: rows of [O, max, sum]
@@ -786,15 +900,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
       }
     }
     __syncthreads();
-    const int64_t w_first = unit0 / sh.per, w_last = (unit0 + en.tiles - 1) / sh.per;
-    const bool alone = w_first == w_last;
+    const bool alone = pc.count == 1;
     const int rows_here = en.r1 - en.r0;
     constexpr int kPieces = D / 4;
     constexpr int kSlot = M * G::kPitch;                 // floats of a partial
-    const int slots = 2 * groups;
     const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
-        a.part, (short)0, (int)min((int64_t)slots * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
-    const int my_slot = 2 * wg + (sh.per * wg < unit0 ? 1 : 0);
+        a.part, (short)0, (int)min((int64_t)a.partials * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
     // O = sum_i (w_i / sum w) O_i with w_i = 2^(m_i - max m) l_i, over the waves
     for (int i = (int)threadIdx.x; i < rows_here * kPieces; i += 256) {
       const int r = i / kPieces, d = i % kPieces * 4;
@@ -818,20 +929,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
         if (a.lse && d == 0)
           a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] = lse_of(mx, l);
       } else {
-        const int at = (my_slot * kSlot + r * G::kPitch) * 4;
+        const int at = (pc.slot * kSlot + r * G::kPitch) * 4;
         store_partial(pr, at + 4 * d, o);
         if (d == 0) store_partial(pr, at + 4 * D, float4_t{mx, l, 0.0f, 0.0f});
       }
     }
     if (!alone) {
-      int32_t* counter = a.counters + w_first;
-      if (arrive_last(counter, (int)(w_last - w_first + 1), &s_last)) {
-        merge_partials<D, M, 256, 1, 16>(a, en, head, unit0, sh.per, w_first, w_last, pr);
+      const int first = pc.slot - pc.at;
+      int32_t* counter = a.counters + first;
+      if (arrive_last(counter, pc.count, &s_last)) {
+        merge_partials<D, M, 256, 1, 16>(a, en, head, [](int w) { return w; }, first, first + pc.count - 1, pr);
         reset_counter(counter);
       }
     }
-
-    next_entry(a, sh, unit0, t1, en.tiles, M);
   }
 #endif
 }
@@ -864,11 +974,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = PrefillGeo<D>;
   constexpr int M = G::kM, kPitch = D + 4, kSlot = M * kPitch;
-  extern __shared__ uint8_t s_stage[];
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_stage[];   // (ds_read_b128 off 16 bytes takes thrice as long)
   __shared__ int s_last;
   // whether a stage's V holds a NaN that some rows see and others do not, and where: [stage][dim][4 blocks of 16 keys]
   __shared__ int s_nan[3];
-  __shared__ uint16_t s_where[2][D][4];
+  __shared__ __attribute__((aligned(16))) uint16_t s_where[2][D][4];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane & 31, hf = lane >> 5;
   const int groups = (int)gridDim.x;
@@ -878,10 +988,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
   if (tid < 3) s_nan[tid] = 0;
 
   while (sh.pos < sh.end) {
-    const int64_t e_id = ((int64_t)__builtin_amdgcn_readfirstlane((int)(sh.entry >> 32)) << 32) |
-                         (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.entry);
-    const Entry en = entry_at(a, e_id, M);
-    const int64_t unit0 = sh.head * sh.per_head + sh.entry_pos;
+    // (uniform over the workgroup, and told so: the loads of an entry then go through the scalar cache)
+    const Entry en = entry_at(a, __builtin_amdgcn_readfirstlane(sh.entry), M);
+    const int64_t unit0 = (int64_t)sh.head * sh.per_head + sh.entry_pos;
     const int t0 = (int)(sh.pos - unit0);
     const int t1 = (int)min((int64_t)en.tiles, sh.end - unit0);
     const int head = sh.head;
@@ -905,35 +1014,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
       }
     }
     const int p_lo = en.start + en.r0 / a.group, p_hi = en.start + (en.r1 - 1) / a.group;
-    const int32_t* row_table = a.table + (int64_t)en.b * a.table_stride;
     auto key_of = [&](int t) { return kTile * (t < en.sink_tiles ? t : t + en.skip); };
 
     // staging: thread tid holds pieces tid + 256 i of the K block (key = piece / (D / 16)) and of the V block (dimension
     // = piece / 4, 16 keys piece % 4)
+    const int32_t* row_table = a.table + (int64_t)en.b * a.table_stride;
+    const uint8_t *k_base = a.kp + head * a.head_stride, *v_base = a.vp + head * a.head_stride;
+    const uint8_t *k_exps = a.ke + head * a.exp_head_stride, *v_exps = a.ve + head * a.exp_head_stride;
+    const int last = max(en.end - 1, 0);            // keys past it look its page up, and are masked
     uint4 kw[G::kLoads], vw[G::kLoads];
-    int kexp[G::kLoads], vexp = -1;
-    const int last = max(en.end - 1, 0);            // keys past it look its page up again, and are masked
+    int kid[G::kLoads], vid = 0;                    // pages of the tile to load next
+    int kexp[G::kLoads], vexp = 0;                  // exponents of the tile to stage
+    bool vok = false;                               // whether its V block holds anything
+    auto pages_at = [&](int t) {
+      const int base = key_of(t);
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i)
+        kid[i] = row_table[min(base + (tid + 256 * i) / (D / 16), last) >> a.page_shift];
+      vid = row_table[min(base + 16 * (tid & 3), last) >> a.page_shift];        // this thread's V keys
+    };
     auto load = [&](int t) {
       const int base = key_of(t);
 #pragma unroll
       for (int i = 0; i < G::kLoads; ++i) {
-        const int piece = tid + 256 * i, key = base + piece / (D / 16);
-        const int id = row_table[min(key, last) >> a.page_shift];
-        const int64_t page = (uint32_t)id < (uint32_t)a.pages ? id : 0;
-        kw[i] = *reinterpret_cast<const uint4*>(a.kp + page * a.page_stride + head * a.head_stride +
-                                                (int64_t)(key & page_mask) * D + piece % (D / 16) * 16);
-        kexp[i] = a.ke[page * a.exp_page_stride + head * a.exp_head_stride];
+        const int piece = tid + 256 * i;
+        const uint32_t page = (uint32_t)kid[i] < a.pages ? kid[i] : 0;
+        kw[i] = *reinterpret_cast<const uint4*>(k_base + (uint64_t)page * a.page_stride +
+                                                (((base + piece / (D / 16)) & page_mask) * D + piece % (D / 16) * 16));
+        kexp[i] = k_exps[(uint64_t)page * a.exp_page_stride];
       }
-      const int key = base + 16 * (tid & 3);       // this thread's V keys, and the block whose exponent it reads
-      const int id = row_table[min(key, last) >> a.page_shift];
-      const bool good = ((uint32_t)id < (uint32_t)a.pages) & (key < en.end);
-      const int64_t page = good ? id : 0;
-      const uint8_t* vp = a.vp + page * a.page_stride + head * a.head_stride + (key & page_mask);
+      vok = ((uint32_t)vid < a.pages) & (base + 16 * (tid & 3) < en.end);
+      const uint32_t page = vok ? vid : 0;
+      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride +
+                          (((tid >> 2) << a.page_shift) + ((base + 16 * (tid & 3)) & page_mask));
 #pragma unroll
-      for (int i = 0; i < G::kLoads; ++i)
-        vw[i] = *reinterpret_cast<const uint4*>(vp + ((int64_t)((tid >> 2) + 64 * i) << a.page_shift));
-      vexp = a.ve[page * a.exp_page_stride + head * a.exp_head_stride];
-      if (!good) vexp = -1;
+      for (int i = 0; i < G::kLoads; ++i) vw[i] = *reinterpret_cast<const uint4*>(vp + ((64 * i) << a.page_shift));
+      vexp = v_exps[(uint64_t)page * a.exp_page_stride];
     };
     int e_ref = 0;                                  // the exponent that O is held at once the staged tile is added
     float e_drop = 1.0f;                            // and what O is multiplied by before that
@@ -944,7 +1060,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     };
     auto stage = [&](int t, int buf, int flag) {
       const int base = key_of(t);
-      const uint32_t ok4 = (uint32_t)__ballot(vexp >= 0) & 15u;
+      const uint32_t ok4 = (uint32_t)__ballot(vok) & 15u;
       block_ok = ok4;
       uint8_t* sk = s_stage + buf * (G::kStageK + G::kStageV);
       uint8_t* sv = sk + G::kStageK;
@@ -959,7 +1075,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
           any |= widest.sees(i) ? 1u << i : 0u;
           all |= least.sees(i) ? 1u << i : 0u;
         }
-        if (vexp < 0) any = 0;
+        if (!vok) any = 0;
         if (any == 0) ev = -1;
         const uint32_t some = any & ~all;
         uint32_t nan = 0;
@@ -1008,7 +1124,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     __syncthreads();        // the stages' and flags' earlier readers are done
     if (tid < 3) s_nan[tid] = 0;
     __syncthreads();
+    pages_at(t0);
     load(t0);
+    if (t0 + 1 < t1) pages_at(t0 + 1);
     stage(t0, 0, 0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -1017,6 +1135,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
       const float drop = e_drop;
       const uint32_t tile_ok = block_ok;
       if (more) load(t + 1);
+      if (t + 2 < t1) pages_at(t + 2);
       const int slot = (t - t0) % 3;
       if (wave_live) {
         const int base = key_of(t);
@@ -1109,17 +1228,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
 
     // every wave has its rows whole: outputs or partials straight from registers (acc[dt][4 a + i] is dimension
     // 32 dt + 8 a + 4 hf + i)
-    const int64_t w_first = unit0 / sh.per, w_last = (unit0 + en.tiles - 1) / sh.per;
+    const int w_first = (int)(unit0 / sh.per), w_last = (int)((unit0 + en.tiles - 1) / sh.per);
     const bool alone = w_first == w_last;
+    // a workgroup's partials: of an entry that began before its run, and of one that ends after it
+    auto slot_of = [&](int w) { return 2 * w + ((int64_t)sh.per * w < unit0 ? 1 : 0); };
     const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
-        a.part, (short)0, (int)min((int64_t)2 * groups * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
+        a.part, (short)0, (int)min((int64_t)a.partials * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
     float l = l_run;
     {
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
       l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     }
     const float f = l != 0.0f ? exp_bits(e_ref) / l : 0.0f;
-    const int my_slot = 2 * wg + (sh.per * wg < unit0 ? 1 : 0);
+    const int my_slot = slot_of(wg);
     if (live) {
 #pragma unroll
       for (int dt = 0; dt < G::kDT; ++dt)
@@ -1140,8 +1261,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     }
     if (!alone) {
       int32_t* counter = a.counters + w_first;
-      if (arrive_last(counter, (int)(w_last - w_first + 1), &s_last)) {
-        merge_partials<D, M, 256, 4, 4>(a, en, head, unit0, sh.per, w_first, w_last, pr);
+      if (arrive_last(counter, w_last - w_first + 1, &s_last)) {
+        merge_partials<D, M, 256, 4, 4>(a, en, head, slot_of, w_first, w_last, pr);
         reset_counter(counter);
       }
     }
@@ -1155,23 +1276,38 @@ int page_shift_of(int page_size) {
                                                                                     : -1;
 }
 
-// The workgroups of a launch (a multiple of 8): two to a CU.
-int attention_groups() { return 2 * device_cus() / 8 * 8; }
-
-constexpr size_t kAttnCounterBytes = 16384;   // arrival counters, one per workgroup (at most 4096)
-
 // Query rows of a workgroup, by the rows (tokens x heads of a group) that a request has on average: 16 or 32 in the
 // decode kernel, which reads its keys from memory wave by wave, else the prefill kernel's 128.
-int tile_rows(int rows, int batch, int group) {
-  const int64_t all = (int64_t)rows * group;
+int tile_rows(int64_t rows, int batch, int group) {
+  const int64_t all = rows * group;
   return all <= 16 * (int64_t)batch ? 16 : all <= 32 * (int64_t)batch ? 32 : 128;
 }
 
-constexpr int kMinTiles = 4;   // key tiles of a workgroup: one for each wave of the decode kernel
+constexpr int64_t kMaxRows = 1 << 30;   // rows x heads of a group: 32-bit row numbers in the kernels
+constexpr int kMinTiles = 4;   // key tiles of a workgroup at least: one for each wave of the decode kernel
 
-size_t attention_workspace(int rows, int batch, int group, int dim) {
-  return kAttnCounterBytes + (size_t)attention_groups() * 2 * tile_rows(rows, batch, group) * (dim + 4) * 4;
+struct Launch {
+  int m, entries, slots, groups;
+  int partials;                // of m rows each
+};
+
+// Workgroups on the CUs at once: two of 4 waves to a CU. The prefill kernel has one workgroup to a slot, each with at
+// most two partials. The decode kernel has as many pieces as slots, or one for each (head, entry) and `sure` more a head
+// (piece_of); those with partials, of entries longer than a size that goes at most `room` times into their sum, are
+// fewer than twice that.
+Launch plan_launch(int rows, int batch, int heads, int group, bool ragged) {
+  Launch x;
+  x.m = tile_rows(rows, batch, group);
+  x.entries = ragged ? (int)((int64_t)rows * group / x.m) + batch : batch * ((group + x.m - 1) / x.m);
+  x.slots = 2 * device_cus() / 8 * 8;
+  const int64_t units = (int64_t)x.entries * heads, room = x.slots > heads ? x.slots : heads;
+  const int64_t most = x.m == 128 ? x.slots : units + room;
+  x.groups = (int)((most + 7) / 8 * 8);
+  x.partials = (int)(x.m == 128 ? 2 * x.slots : 2 * room);
+  return x;
 }
+
+size_t counter_bytes(const Launch& x) { return ((size_t)x.partials * 4 + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace xt
@@ -1197,6 +1333,8 @@ static int check_pool(const char* what, const void* k, const void* vt, const voi
       *page_stride < block || *exp_head_stride < 1 || *exp_page_stride < 1)
     return fail(XT_EINVAL, "%s: blocks must be 16-byte aligned and %lld bytes or more apart (page stride %lld, head "
                 "stride %lld)", what, (long long)block, (long long)*page_stride, (long long)*head_stride);
+  if (*page_stride > 0xFFFFFFFFll || *exp_page_stride > 0xFFFFFFFFll)
+    return fail(XT_EUNSUPPORTED, "%s: pages %lld bytes apart", what, (long long)*page_stride);
   return XT_OK;
 }
 
@@ -1239,8 +1377,14 @@ extern "C" int xt_page8_append(const void* k, int64_t k_row_stride, int64_t k_he
 }
 
 extern "C" size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_heads, int kv_heads, int dim) {
-  if (rows < 0 || batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || dim < 1) return 0;
-  return attention_workspace(rows, batch, q_heads / kv_heads, dim);
+  if (rows < 0 || batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || dim < 1 ||
+      (int64_t)rows * (q_heads / kv_heads) > kMaxRows || (int64_t)batch * q_heads > kMaxRows)
+    return 0;
+  const Launch x = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, true);
+  const Launch y = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, false);
+  const size_t partial = (size_t)x.m * (dim + 4) * 4;
+  const size_t a = counter_bytes(x) + x.partials * partial, b = counter_bytes(y) + y.partials * partial;
+  return a > b ? a : b;
 }
 
 template <int D, int NQ>
@@ -1283,26 +1427,29 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
   if (out_dtype != XT_DTYPE_BF16 && out_dtype != XT_DTYPE_F16)
     return fail(XT_EINVAL, "%s: output type %d", what, out_dtype);
   if (rows == 0 || batch == 0) return ok();
-  if ((int64_t)rows * group > 0x7FFFFFFF / 2)
-    return fail(XT_EUNSUPPORTED, "%s: %d rows x %d heads of a group", what, rows, group);
+  if ((int64_t)rows * group > kMaxRows || (int64_t)batch * q_heads > kMaxRows)
+    return fail(XT_EUNSUPPORTED, "%s: %d rows, %d requests, %d query heads", what, rows, batch, q_heads);
   if (const int st = check_rows(what, table, table_stride, width, seq_lens, cu_q, batch, rows)) return st;
   if (!q || !out || !aligned(q, 16) || q_row_stride % 8 || q_head_stride % 8 || !aligned(out, 8) ||
       out_row_stride % 4 || out_head_stride % 4)
     return fail(XT_EINVAL, "%s: query rows must be 16-byte aligned, output rows 8-byte aligned", what);
-  const size_t need = attention_workspace(rows, batch, group, dim);
+  const Launch x = plan_launch(rows, batch, kv_heads, group, cu_q != nullptr);
+  const int64_t tiles = ((int64_t)width * page_size + kTile - 1) / kTile;    // of an entry at most
+  if (tiles > 0x7FFFFFFF / x.entries || tiles * x.entries > ((int64_t)1 << 38) / kv_heads)
+    return fail(XT_EUNSUPPORTED, "%s: %d row tiles over a table of %d pages", what, x.entries, width);
+  const size_t need = counter_bytes(x) + x.partials * (size_t)x.m * (dim + 4) * 4;
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, workspace_bytes, need);
-  const int m = tile_rows(rows, batch, group);
-  const int64_t entries = cu_q ? (int64_t)rows * group / m + batch : (int64_t)batch * ((group + m - 1) / m);
   // no more workgroups than the table's width could keep busy
-  const int64_t most = entries * kv_heads * ((((int64_t)width * page_size + kTile - 1) / kTile + kMinTiles - 1) / kMinTiles);
-  int groups = attention_groups();
-  if (most < groups) groups = (int)((most + 7) / 8 * 8);
-  AttnArgs a{(const uint16_t*)q, q_row_stride, q_head_stride, k_pages, vt_pages, k_exp, v_exp, page_stride,
-             head_stride, exp_page_stride, exp_head_stride, pages, page_shift_of(page_size), kv_heads, group, table,
+  const int64_t most = (int64_t)x.entries * kv_heads * ((tiles + kMinTiles - 1) / kMinTiles);
+  const int groups = most < x.groups ? (int)((most + 7) / 8 * 8) : x.groups;
+  AttnArgs a{(const uint16_t*)q, q_row_stride, q_head_stride, k_pages, vt_pages, k_exp, v_exp, (uint32_t)page_stride,
+             (uint32_t)exp_page_stride, head_stride, exp_head_stride, (uint32_t)pages, page_shift_of(page_size), kv_heads,
+             group, table,
              table_stride, width, seq_lens, cu_q, batch, rows, window, sinks, scale * kLog2e, out, out_row_stride,
-             out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse, entries, kMinTiles,
-             (int32_t*)workspace, (float*)((uint8_t*)workspace + kAttnCounterBytes)};
+             out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse, x.entries, kMinTiles, x.slots,
+             (int32_t*)workspace, (float*)((uint8_t*)workspace + counter_bytes(x)), x.partials};
+  const int m = x.m;
   if (m == 16) {
     if (dim == 64) return launch_decode<64, 1>(what, a, groups, stream);
     if (dim == 128) return launch_decode<128, 1>(what, a, groups, stream);

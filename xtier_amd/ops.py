@@ -5,7 +5,6 @@ xtier/backend/formats.py). Tensors are torch tensors on the GPU; every call runs
 ``raw`` is the reference's tuple of a layer's pool buffers (qsa_fp4.py:43-58):
 (k_pay u8 [slots, kv_heads, dim/2], v_pay, k_scales u8 [slots, kv_heads, dim/16], v_scales, gk f32 [1], gv f32 [1]).
 """
-import contextlib
 import ctypes
 import functools
 import math
@@ -1130,48 +1129,53 @@ def minimax_prefill_scores(q, idx_pay, idx_sc, req_to_token, score, cu_seqlens, 
 
 # --- the 8-bit paged cache ------------------------------------------------------------------------------------------
 
-def _one_device(what, *tensors):
-    """Every given tensor is on one GPU. Returns a context that makes it the current one."""
-    first = None
+def _away(what, *tensors):
+    """Checks that the given tensors are on one GPU; returns its index if that is not the current one, else None."""
+    first = -2                    # (a CPU tensor's index is -1)
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError('xtier_amd: GPU tensors expected')
-        if first is None:
-            first = t.get_device()
-        elif t.get_device() != first:
-            raise ValueError(f'xtier_amd.{what}: tensors on cuda:{first} and cuda:{t.get_device()}')
-    return contextlib.nullcontext() if first == torch.cuda.current_device() else torch.cuda.device(first)
+        if t is not None:
+            d = t.get_device()
+            if d != first:
+                if d < 0:
+                    raise ValueError('xtier_amd: GPU tensors expected')
+                if first >= 0:
+                    raise ValueError(f'xtier_amd.{what}: tensors on cuda:{first} and cuda:{d}')
+                first = d
+    return None if first == torch._C._cuda_getDevice() else first
 
 
 def _int32(t):
-    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+    return t if t is None or (t.dtype is torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+
+
+_E4M3_BYTES = (torch.uint8, torch.float8_e4m3fn)
 
 
 def _check_page8(what, raw):
     """The pool tuple of the 8-bit pages: (k [pages, heads, page, dim], vt [pages, heads, dim, page], k_exp, v_exp
-    [pages, heads]), bytes; each block contiguous, pages and heads strided alike for K and V."""
+    [pages, heads]), bytes; each block contiguous, pages and heads strided alike for K and V. Returns the addresses and
+    sizes, head size, page size and strides of the C call."""
     k, vt, k_exp, v_exp = raw
-    if k.dim() != 4 or vt.dim() != 4 or k_exp.dim() != 2:
-        raise ValueError(f'xtier_amd.{what}: blocks [pages, heads, page, dim] and scales [pages, heads] expected')
-    pages, heads, page, dim = k.shape
-    ks, vs, es = k.stride(), vt.stride(), k_exp.stride()
-    if (k.element_size() != 1 or vt.element_size() != 1 or k_exp.dtype != torch.uint8 or v_exp.dtype != torch.uint8
-            or vt.shape != (pages, heads, dim, page) or k_exp.shape != (pages, heads) or v_exp.shape != (pages, heads)
-            or ks[3] != 1 or ks[2] != dim or vs[3] != 1 or vs[2] != page or ks[:2] != vs[:2] or v_exp.stride() != es):
-        raise ValueError(f'xtier_amd.{what}: an 8-bit pool of blocks k [pages, heads, page, dim], vt [pages, heads, dim, '
-                         f'page] and scales [pages, heads] expected, got {tuple(k.shape)} {ks}, {tuple(vt.shape)} {vs}, '
-                         f'{tuple(k_exp.shape)} {es}')
-    return (k.data_ptr(), vt.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), pages, heads), dim, page, \
-        (ks[0], ks[1], es[0], es[1])
+    shape, ks, es = k.shape, k.stride(), k_exp.stride()
+    if len(shape) == 4:
+        pages, heads, page, dim = shape
+        if (ks[3] == 1 and ks[2] == dim and vt.shape == (pages, heads, dim, page) and k_exp.shape == shape[:2]
+                and vt.stride() == (ks[0], ks[1], page, 1) and v_exp.shape == shape[:2] and v_exp.stride() == es
+                and k.dtype in _E4M3_BYTES and vt.dtype in _E4M3_BYTES and k_exp.dtype is torch.uint8
+                and v_exp.dtype is torch.uint8):
+            return ((k.data_ptr(), vt.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), pages, heads), dim, page,
+                    (ks[0], ks[1], es[0], es[1]))
+    raise ValueError(f'xtier_amd.{what}: an 8-bit pool of blocks k [pages, heads, page, dim], vt [pages, heads, dim, '
+                     f'page] (E4M3) and scales [pages, heads] (uint8) expected, got {tuple(shape)} {ks} {k.dtype}, '
+                     f'{tuple(vt.shape)} {vt.stride()}, {tuple(k_exp.shape)} {es} {k_exp.dtype}')
 
 
 def _page_table(what, table, seq_lens, cu, rows):
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+    shape = table.shape
+    if len(shape) != 2 or table.dtype is not torch.int32 or (table.stride(1) != 1 and shape[1] > 1):
         raise ValueError(f'xtier_amd.{what}: an int32 page table [requests, pages] with contiguous rows expected')
-    batch = table.shape[0]
-    if seq_lens.numel() != batch or (cu is not None and cu.numel() != batch + 1) or (cu is None and rows != batch):
+    batch = shape[0]
+    if seq_lens.numel() != batch or (rows != batch if cu is None else cu.numel() != batch + 1):
         raise ValueError(f'xtier_amd.{what}: {rows} rows, {seq_lens.numel()} lengths, '
                          f'{None if cu is None else cu.numel()} row offsets for a table of {batch} requests')
     return batch
@@ -1184,18 +1188,23 @@ def page8_append(k, v, raw, table, seq_lens, cu_rows=None):
     positions. Each page and head keeps a power-of-two scale, which grows with its largest value (see
     xt_page8_append); no page may take rows of two requests."""
     ptrs, dim, page, strides = _check_page8('page8_append', raw)
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 3 or k.shape != v.shape \
-            or k.shape[1:] != (ptrs[5], dim) or k.stride(2) != 1 or v.stride(2) != 1:
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or v.shape != shape \
+            or shape[1:] != (ptrs[5], dim) or ks[2] != 1 or vs[2] != 1:
         raise ValueError(f'xtier_amd.page8_append: BF16 rows [rows, {ptrs[5]}, {dim}] expected, got {k.dtype} '
                          f'{tuple(k.shape)}, {v.dtype} {tuple(v.shape)}')
-    rows = k.shape[0]
-    batch = _page_table('page8_append', table, seq_lens, cu_rows, rows)
-    with _one_device('page8_append', k, v, *raw, table, seq_lens, cu_rows):
-        seq_lens, cu_rows = _int32(seq_lens), _int32(cu_rows)
-        _lib.check(_lib.lib().xt_page8_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), rows, *ptrs, dim, page,
-            *strides, table.data_ptr(), table.stride(0), table.shape[1], seq_lens.data_ptr(), _ptr(cu_rows), batch,
-            _stream(k)), 'page8_append')
+    batch = _page_table('page8_append', table, seq_lens, cu_rows, shape[0])
+    away = _away('page8_append', k, v, *raw, table, seq_lens, cu_rows)
+    if away is not None:
+        with torch.cuda.device(away):
+            return page8_append(k, v, raw, table, seq_lens, cu_rows)
+    seq_lens, cu_rows = _int32(seq_lens), _int32(cu_rows)
+    st = _lib.lib().xt_page8_append(
+        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], shape[0], *ptrs, dim, page, *strides, table.data_ptr(),
+        table.stride(0), table.shape[1], seq_lens.data_ptr(), None if cu_rows is None else cu_rows.data_ptr(), batch,
+        _stream(k))
+    if st:
+        _lib.check(st, 'page8_append')
 
 
 _stream_workspaces = {}   # (device index, stream) -> zeroed uint8 tensor
@@ -1205,11 +1214,11 @@ def _stream_workspace(t, nbytes):
     """A zero-filled workspace for a call on t's device and its current stream: kept per stream, so calls that overlap
     on two streams never share one; inside a graph capture a new one of the graph's own memory, so graphs never share
     one either."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=t.device)
     key = (t.get_device(), _stream(t))
     buf = _stream_workspaces.get(key)
-    if buf is None or buf.numel() < nbytes:
+    if buf is None or buf.shape[0] < nbytes:
         buf = _stream_workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=t.device)
     return buf
 
@@ -1226,27 +1235,38 @@ def page8_attention(q, raw, table, seq_lens, scale, cu_q=None, window=0, sinks=0
     and the first ``sinks``. Returns out [rows, q_heads, dim] (BF16 unless ``out`` is given, BF16 or FP16); lse FP32
     [rows, q_heads] is filled if given. ws: a zero-filled workspace of page8_workspace_bytes, None (one per stream)."""
     ptrs, dim, page, strides = _check_page8('page8_attention', raw)
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != dim or q.stride(2) != 1:
+    shape, qs = q.shape, q.stride()
+    if q.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != dim or qs[2] != 1:
         raise ValueError(f'xtier_amd.page8_attention: BF16 queries [rows, heads, {dim}] expected, got {q.dtype} '
-                         f'{tuple(q.shape)}')
-    rows, q_heads = q.shape[:2]
+                         f'{tuple(shape)}')
+    rows, q_heads = shape[0], shape[1]
     batch = _page_table('page8_attention', table, seq_lens, cu_q, rows)
-    with _one_device('page8_attention', q, *raw, table, seq_lens, cu_q, out, lse, ws):
-        if out is None:
-            out = torch.empty((rows, q_heads, dim), dtype=torch.bfloat16, device=q.device)
-        if out.dtype not in _DTYPES or out.shape != q.shape or out.stride(2) != 1:
-            raise ValueError(f'xtier_amd.page8_attention: a BF16 or FP16 output {tuple(q.shape)} with a contiguous last '
+    away = _away('page8_attention', q, *raw, table, seq_lens, cu_q, out, lse, ws)
+    if away is not None:
+        with torch.cuda.device(away):
+            return page8_attention(q, raw, table, seq_lens, scale, cu_q, window, sinks, out, lse, ws)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        os, out_dtype = out.stride(), _lib.XT_DTYPE_BF16
+    else:
+        os, out_dtype = out.stride(), _DTYPES.get(out.dtype)
+        if out_dtype is None or out.shape != shape or os[2] != 1:
+            raise ValueError(f'xtier_amd.page8_attention: a BF16 or FP16 output {tuple(shape)} with a contiguous last '
                              f'dim expected, got {out.dtype} {tuple(out.shape)}')
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
-            raise ValueError(f'xtier_amd.page8_attention: a contiguous FP32 lse {tuple(q.shape[:2])} expected')
-        if ws is None:
-            ws = _stream_workspace(q, page8_workspace_bytes(rows, batch, q_heads, ptrs[5], dim) if batch else 256)
-        seq_lens, cu_q = _int32(seq_lens), _int32(cu_q)
-        _lib.check(_lib.lib().xt_page8_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), *ptrs, q_heads, dim, page, *strides, table.data_ptr(),
-            table.stride(0), table.shape[1], seq_lens.data_ptr(), _ptr(cu_q), batch, rows, int(window), int(sinks),
-            float(scale), out.data_ptr(), out.stride(0), out.stride(1), _DTYPES[out.dtype], _ptr(lse), ws.data_ptr(),
-            ws.numel(), _stream(q)), 'page8_attention')
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
+        raise ValueError(f'xtier_amd.page8_attention: a contiguous FP32 lse {tuple(shape[:2])} expected')
+    if ws is not None and ws.dtype is not torch.uint8:
+        raise ValueError('xtier_amd.page8_attention: a uint8 workspace expected')
+    if ws is None:
+        ws = _stream_workspace(q, page8_workspace_bytes(rows, batch, q_heads, ptrs[5], dim) if batch else 256)
+    seq_lens, cu_q = _int32(seq_lens), _int32(cu_q)
+    st = _lib.lib().xt_page8_attention(
+        q.data_ptr(), qs[0], qs[1], *ptrs, q_heads, dim, page, *strides, table.data_ptr(), table.stride(0),
+        table.shape[1], seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, rows, int(window),
+        int(sinks), float(scale), out.data_ptr(), os[0], os[1], out_dtype, None if lse is None else lse.data_ptr(),
+        ws.data_ptr(), ws.numel(), _stream(q))
+    if st:
+        _lib.check(st, 'page8_attention')
     return out
 
 
@@ -1274,12 +1294,15 @@ def pages_extend(refs, table, lens, add, page_size):
     pages, stride, width, rows = _check_pages('pages_extend', refs, table, lens)
     if add.shape != lens.shape:
         raise ValueError(f'xtier_amd.pages_extend: {add.numel()} sizes for {rows} rows')
-    with _one_device('pages_extend', refs, table, lens, add):
-        granted = torch.empty(rows, dtype=torch.bool, device=refs.device)
-        ws, add = _pages_workspace(refs), _int32(add)
-        _lib.check(_lib.lib().xt_pages_extend(
-            _ptr(refs), pages, _ptr(table), stride, width, _ptr(lens), _ptr(add), rows, int(page_size), _ptr(granted),
-            _ptr(ws), ws.numel() * 4, _stream(refs)), 'pages_extend')
+    away = _away('pages_extend', refs, table, lens, add)
+    if away is not None:
+        with torch.cuda.device(away):
+            return pages_extend(refs, table, lens, add, page_size)
+    granted = torch.empty(rows, dtype=torch.bool, device=refs.device)
+    ws, add = _pages_workspace(refs), _int32(add)
+    _lib.check(_lib.lib().xt_pages_extend(
+        refs.data_ptr(), pages, table.data_ptr(), stride, width, lens.data_ptr(), add.data_ptr(), rows, int(page_size),
+        granted.data_ptr(), ws.data_ptr(), ws.shape[0] * 4, _stream(refs)), 'pages_extend')
     return granted
 
 
@@ -1291,13 +1314,17 @@ def pages_fork(refs, table, lens, parents, children, page_size):
     pages, stride, width, rows = _check_pages('pages_fork', refs, table, lens)
     if parents.dim() != 1 or parents.shape != children.shape:
         raise ValueError('xtier_amd.pages_fork: as many parents as children expected')
+    away = _away('pages_fork', refs, table, lens, parents, children)
+    if away is not None:
+        with torch.cuda.device(away):
+            return pages_fork(refs, table, lens, parents, children, page_size)
     n = parents.shape[0]
-    with _one_device('pages_fork', refs, table, lens, parents, children):
-        moves = torch.empty((2, n), dtype=torch.int32, device=refs.device)
-        ws, parents, children = _pages_workspace(refs, n), _int32(parents), _int32(children)
-        _lib.check(_lib.lib().xt_pages_fork(
-            _ptr(refs), pages, _ptr(table), stride, width, _ptr(lens), rows, int(page_size), _ptr(parents),
-            _ptr(children), n, _ptr(moves), n, _ptr(ws), ws.numel() * 4, _stream(refs)), 'pages_fork')
+    moves = torch.empty((2, n), dtype=torch.int32, device=refs.device)
+    ws, parents, children = _pages_workspace(refs, n), _int32(parents), _int32(children)
+    _lib.check(_lib.lib().xt_pages_fork(
+        refs.data_ptr(), pages, table.data_ptr(), stride, width, lens.data_ptr(), rows, int(page_size),
+        parents.data_ptr(), children.data_ptr(), n, moves.data_ptr(), n, ws.data_ptr(), ws.shape[0] * 4,
+        _stream(refs)), 'pages_fork')
     return moves
 
 
@@ -1305,10 +1332,13 @@ def pages_free(refs, table, lens, rows):
     """Frees the table rows ``rows`` (int32 ids; one named twice is freed once): their pages lose a reference, their
     entries become -1 and their lengths 0, in place."""
     pages, stride, width, n_rows = _check_pages('pages_free', refs, table, lens)
-    with _one_device('pages_free', refs, table, lens, rows):
-        rows = _int32(rows)
-        _lib.check(_lib.lib().xt_pages_free(_ptr(refs), pages, _ptr(table), stride, width, _ptr(lens), n_rows,
-                                            _ptr(rows), rows.numel(), _stream(refs)), 'pages_free')
+    away = _away('pages_free', refs, table, lens, rows)
+    if away is not None:
+        with torch.cuda.device(away):
+            return pages_free(refs, table, lens, rows)
+    rows = _int32(rows)
+    _lib.check(_lib.lib().xt_pages_free(refs.data_ptr(), pages, table.data_ptr(), stride, width, lens.data_ptr(), n_rows,
+                                        rows.data_ptr(), rows.numel(), _stream(refs)), 'pages_free')
 
 
 def pages_compact(refs, table):
@@ -1316,18 +1346,22 @@ def pages_compact(refs, table):
     below L. refs and table follow in place. Returns (moves int32 [2, pages // 2], count int32 [1]): the first count
     columns are the pages (from, to) that pages_copy has to copy in every layer, -1 behind them."""
     pages, stride, width, rows = _check_pages('pages_compact', refs, table)
-    with _one_device('pages_compact', refs, table):
-        moves = torch.empty((2, pages // 2), dtype=torch.int32, device=refs.device)
-        count = torch.empty(1, dtype=torch.int32, device=refs.device)
-        ws = _pages_workspace(refs)
-        _lib.check(_lib.lib().xt_pages_compact(_ptr(refs), pages, _ptr(table), stride, width, rows, _ptr(moves),
-                                               _ptr(count), _ptr(ws), ws.numel() * 4, _stream(refs)), 'pages_compact')
+    away = _away('pages_compact', refs, table)
+    if away is not None:
+        with torch.cuda.device(away):
+            return pages_compact(refs, table)
+    moves = torch.empty((2, pages // 2), dtype=torch.int32, device=refs.device)
+    count = torch.empty(1, dtype=torch.int32, device=refs.device)
+    ws = _pages_workspace(refs)
+    _lib.check(_lib.lib().xt_pages_compact(refs.data_ptr(), pages, table.data_ptr(), stride, width, rows,
+                                           moves.data_ptr(), count.data_ptr(), ws.data_ptr(), ws.shape[0] * 4,
+                                           _stream(refs)), 'pages_compact')
     return moves, count
 
 
 class PageBuffers:
     """The page buffers of a cache, for pages_copy: tensors [pages, ...] whose pages are contiguous (any stride between
-    them), of any type and size. A server makes one for all layers."""
+    them), of any type and size, on one GPU. A server makes one for all layers."""
 
     def __init__(self, tensors):
         self.tensors = list(tensors)
@@ -1336,13 +1370,12 @@ class PageBuffers:
             if t.dim() < 1 or not (t.shape[0] == 0 or t[0].is_contiguous()):
                 raise ValueError(f'xtier_amd.PageBuffers: [pages, ...] with contiguous pages expected, got '
                                  f'{tuple(t.shape)} strides {t.stride()}')
-            size = t.element_size()
-            descs.append(_lib.PageBuffer(t.data_ptr(), t.shape[0], t.stride(0) * size,
-                                         math.prod(t.shape[1:]) * size))
-        self.guard_tensors = self.tensors[:1]
-        for t in self.tensors[1:]:
             if t.device != self.tensors[0].device:
                 raise ValueError('xtier_amd.PageBuffers: buffers on one GPU expected')
+            size = t.element_size()
+            if t.numel():
+                descs.append(_lib.PageBuffer(t.data_ptr(), t.shape[0], t.stride(0) * size,
+                                             math.prod(t.shape[1:]) * size))
         most = _lib.PAGES_COPY_MAX
         self.groups = [((_lib.PageBuffer * len(part))(*part), len(part))
                        for part in (descs[i:i + most] for i in range(0, len(descs), most))]
@@ -1354,10 +1387,13 @@ def pages_copy(buffers, moves, count=None):
     outside a buffer's pages are skipped. No destination may be another move's source or destination."""
     if not isinstance(buffers, PageBuffers):
         buffers = PageBuffers(buffers)
-    if moves.dim() != 2 or moves.shape[0] != 2 or moves.dtype != torch.int32 \
-            or (moves.shape[1] > 1 and moves.stride(1) != 1) or (count is not None and count.dtype != torch.int32):
+    if moves.dim() != 2 or moves.shape[0] != 2 or moves.dtype is not torch.int32 \
+            or (moves.shape[1] > 1 and moves.stride(1) != 1) or (count is not None and count.dtype is not torch.int32):
         raise ValueError('xtier_amd.pages_copy: int32 moves [2, n] and an int32 count expected')
-    with _one_device('pages_copy', moves, count, *buffers.guard_tensors):
-        for descs, n in buffers.groups:
-            _lib.check(_lib.lib().xt_pages_copy(descs, n, _ptr(moves), moves.stride(0), moves.shape[1], _ptr(count),
-                                                _stream(moves)), 'pages_copy')
+    away = _away('pages_copy', moves, count, *buffers.tensors[:1])
+    if away is not None:
+        with torch.cuda.device(away):
+            return pages_copy(buffers, moves, count)
+    for descs, n in buffers.groups:
+        _lib.check(_lib.lib().xt_pages_copy(descs, n, moves.data_ptr(), moves.stride(0), moves.shape[1],
+                                            None if count is None else count.data_ptr(), _stream(moves)), 'pages_copy')
