@@ -403,6 +403,9 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
 
 // A workgroup's work in the prefill kernel: tiles pos .. end - 1 of the launch, equal runs for all workgroups, one per
 // slot. They are bound by their arithmetic, so equal runs end together where whole units would leave slots idle.
+//
+// (What is the same in every lane but comes out of LDS goes through readfirstlane, in both kernels: the loads of an entry
+// are then scalar loads, and the loops over tiles and their branches scalar ones.)
 struct Share {
   int per, per_head;              // tiles of a workgroup, of one head
   int64_t total, pos, end;        // tiles of the launch; this workgroup's run
@@ -421,6 +424,7 @@ __device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int 
   int sum = 0, before, all, unused, none;
   for (int e = e0; e < e1; ++e) sum += entry_at(a, e, m_rows).tiles;
   block_sums<T>(sum, 0, s_sum, &before, &all, &unused, &none);
+  all = __builtin_amdgcn_readfirstlane(all);
   sh.per_head = all;
   sh.total = (int64_t)all * a.heads;
   sh.per = (int)((sh.total + groups - 1) / groups);
@@ -444,8 +448,8 @@ __device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int 
     }
   }
   __syncthreads();
-  sh.entry = s_find[0];
-  sh.entry_pos = s_find[1];
+  sh.entry = __builtin_amdgcn_readfirstlane(s_find[0]);
+  sh.entry_pos = __builtin_amdgcn_readfirstlane(s_find[1]);
   return sh;
 }
 
@@ -647,7 +651,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
   constexpr int M = G::kRows;
   extern __shared__ __attribute__((aligned(16))) float s_merge[];
   __shared__ int s_last;
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const Piece pc = piece_of<256>(a, M, (int)blockIdx.x);
   if (pc.count == 0) return;
@@ -950,12 +954,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
 
 // 128 query rows a workgroup, 32 for each of its 4 waves, on 32x32 MFMAs. The workgroup dequantizes each 64-key tile
 // once, K to BF16 and V to FP16, into one of two LDS stages while it computes on the other: a wave's 32 rows alone would
-// pay the conversion four times over. K rows lie in LDS in the order of the A rows of S^T (key_row) and 16-byte units of
-// a row are rotated by an XOR with the row, so that the reads of 8 neighbouring lanes fall into different banks.
+// pay the conversion four times over. K rows lie in LDS in the order of the A rows of S^T (key_row).
 template <int D>
 struct PrefillGeo {
   static constexpr int kM = 128;
-  static constexpr int kStageK = kTile * D * 2, kStageV = D * kTile * 2;
+  // Rows of a stage are padded by 16 bytes: LDS reads 16 lanes' 16-byte units at a time from 64 banks, and 16 rows in a
+  // row, an odd number of units apart, put the same unit at 16 different places. (An XOR of the unit with the row
+  // saves the padding, but costs an address register or instruction for every unit of a row.)
+  static constexpr int kRowK = D * 2 + 16, kRowV = kTile * 2 + 16;
+  static constexpr int kStageK = kTile * kRowK, kStageV = D * kRowV;
   static constexpr int kLds = 2 * (kStageK + kStageV);
   static constexpr int kLoads = kTile * D / 16 / 256;    // 16-byte pieces of K, and of V, that a thread stages: D / 64
   static constexpr int kDT = D / 32;
@@ -969,27 +976,42 @@ __device__ inline int key_row(int key) {
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
-template <int D>
+// Computed at this place: the compiler otherwise moves what is first used in a later block there, away from the MFMAs that
+// it is meant to run beside. (x must be the result of an ordinary vector instruction, as in max2_raw.)
+template <typename T>
+__device__ inline void keep_here(T& x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x));
+#endif
+}
+
+// The step of tile t: S(t + 1) = K(t + 1) Q^T beside the softmax of S(t), then O += V(t) P(t) beside the conversion of
+// K(t + 2) and V(t + 1), which lie in registers, and the loads of the pair after them. MFMAs and vector instructions of
+// one wave alternate, because two waves on a SIMD (what 256 registers allow) do not fill it otherwise: a wave issues an
+// instruction every 8 clocks at most, a vector instruction takes 4 and an MFMA 32. Fences to the scheduler keep that order.
+//
+// ONE: pages of 64 tokens and more, so that a tile lies in one page, whose address is then a scalar.
+template <int D, bool ONE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = PrefillGeo<D>;
-  constexpr int M = G::kM, kPitch = D + 4, kSlot = M * kPitch;
+  constexpr int M = G::kM, kPitch = D + 4, kSlot = M * kPitch, NX = D / 16;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_stage[];   // (ds_read_b128 off 16 bytes takes thrice as long)
   __shared__ int s_last;
   // whether a stage's V holds a NaN that some rows see and others do not, and where: [stage][dim][4 blocks of 16 keys]
   __shared__ int s_nan[3];
   __shared__ __attribute__((aligned(16))) uint16_t s_where[2][D][4];
-  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
   const int groups = (int)gridDim.x;
   const int wg = xcd_order((int)blockIdx.x, groups);
   Share sh = share_of<256>(a, M, groups, wg);
   const int page_mask = (1 << a.page_shift) - 1;
-  if (tid < 3) s_nan[tid] = 0;
+  uint8_t* const s_k = s_stage;                       // [2][64 keys][D] BF16
+  uint8_t* const s_v = s_stage + 2 * G::kStageK;      // [2][D][64 keys] FP16
 
   while (sh.pos < sh.end) {
-    // (uniform over the workgroup, and told so: the loads of an entry then go through the scalar cache)
-    const Entry en = entry_at(a, __builtin_amdgcn_readfirstlane(sh.entry), M);
+    const Entry en = entry_at(a, sh.entry, M);
     const int64_t unit0 = (int64_t)sh.head * sh.per_head + sh.entry_pos;
     const int t0 = (int)(sh.pos - unit0);
     const int t1 = (int)min((int64_t)en.tiles, sh.end - unit0);
@@ -997,24 +1019,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
 
     const int r = en.r0 + 32 * wave + c;
     const bool live = r < en.r1;
-    const bool wave_live = en.r0 + 32 * wave < en.r1;
     const int rr = live ? r : en.r1 - 1;
     const int tok = rr / a.group;
     const int64_t q_row = en.row0 + tok;
     const int q_head = head * a.group + (rr - tok * a.group);
     const int pos = en.start + tok;
-    bf16x8_t qb[D / 16];
+    bf16x8_t qb[NX];
     {
       const uint16_t* src = a.q + q_row * a.q_row + q_head * a.q_head + 8 * hf;
 #pragma unroll
-      for (int x = 0; x < D / 16; ++x) {
+      for (int x = 0; x < NX; ++x) {
         uint4 w = {0, 0, 0, 0};
         if (live) w = *reinterpret_cast<const uint4*>(src + 16 * x);
         qb[x] = __builtin_bit_cast(bf16x8_t, w);
       }
     }
     const int p_lo = en.start + en.r0 / a.group, p_hi = en.start + (en.r1 - 1) / a.group;
-    auto key_of = [&](int t) { return kTile * (t < en.sink_tiles ? t : t + en.skip); };
+    // (tiles past the run repeat its last one: the step loads and multiplies ahead without asking)
+    auto key_of = [&](int t) {
+      const int u = min(t, t1 - 1);
+      return kTile * (u < en.sink_tiles ? u : u + en.skip);
+    };
 
     // staging: thread tid holds pieces tid + 256 i of the K block (key = piece / (D / 16)) and of the V block (dimension
     // = piece / 4, 16 keys piece % 4)
@@ -1023,49 +1048,75 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     const uint8_t *k_exps = a.ke + head * a.exp_head_stride, *v_exps = a.ve + head * a.exp_head_stride;
     const int last = max(en.end - 1, 0);            // keys past it look its page up, and are masked
     uint4 kw[G::kLoads], vw[G::kLoads];
-    int kid[G::kLoads], vid = 0;                    // pages of the tile to load next
-    int kexp[G::kLoads], vexp = 0;                  // exponents of the tile to stage
-    bool vok = false;                               // whether its V block holds anything
-    auto pages_at = [&](int t) {
-      const int base = key_of(t);
+    int kid[ONE ? 1 : G::kLoads], vid = 0;          // pages of the tiles to load next
+    int kexp[ONE ? 1 : G::kLoads], vexp = 0;        // exponents of the tiles to stage
+    bool vok = false;                               // whether the V block holds anything
+    auto k_page = [&](int t) {
+      if constexpr (ONE) {
+        kid[0] = uniform_load(row_table + (min(key_of(t), last) >> a.page_shift));
+      } else {
 #pragma unroll
-      for (int i = 0; i < G::kLoads; ++i)
-        kid[i] = row_table[min(base + (tid + 256 * i) / (D / 16), last) >> a.page_shift];
-      vid = row_table[min(base + 16 * (tid & 3), last) >> a.page_shift];        // this thread's V keys
+        for (int i = 0; i < G::kLoads; ++i)
+          kid[i] = row_table[min(key_of(t) + (tid + 256 * i) / (D / 16), last) >> a.page_shift];
+      }
     };
-    auto load = [&](int t) {
+    auto v_page = [&](int t) {
+      if constexpr (ONE) vid = uniform_load(row_table + (min(key_of(t), last) >> a.page_shift));
+      else vid = row_table[min(key_of(t) + 16 * (tid & 3), last) >> a.page_shift];
+    };
+    // one byte by a scalar load of the word that holds it
+    auto scalar_byte = [](const uint8_t* p) {
+      const uint64_t at = (uint64_t)p;
+      return uniform_load(reinterpret_cast<const int32_t*>(at & ~(uint64_t)3)) >> (8 * (int)(at & 3)) & 0xFF;
+    };
+    auto load_k = [&](int t, int i) {
       const int base = key_of(t);
-#pragma unroll
-      for (int i = 0; i < G::kLoads; ++i) {
+      const int32_t id = kid[ONE ? 0 : i];
+      const uint32_t page = (uint32_t)id < a.pages ? id : 0;
+      if constexpr (ONE) {
+        const uint8_t* block = k_base + (uint64_t)page * a.page_stride + (uint32_t)((base & page_mask) * D);
+        kw[i] = *reinterpret_cast<const uint4*>(block + (uint32_t)(tid * 16) + 4096 * i);
+      } else {
         const int piece = tid + 256 * i;
-        const uint32_t page = (uint32_t)kid[i] < a.pages ? kid[i] : 0;
         kw[i] = *reinterpret_cast<const uint4*>(k_base + (uint64_t)page * a.page_stride +
                                                 (((base + piece / (D / 16)) & page_mask) * D + piece % (D / 16) * 16));
         kexp[i] = k_exps[(uint64_t)page * a.exp_page_stride];
       }
-      vok = ((uint32_t)vid < a.pages) & (base + 16 * (tid & 3) < en.end);
-      const uint32_t page = vok ? vid : 0;
-      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride +
-                          (((tid >> 2) << a.page_shift) + ((base + 16 * (tid & 3)) & page_mask));
-#pragma unroll
-      for (int i = 0; i < G::kLoads; ++i) vw[i] = *reinterpret_cast<const uint4*>(vp + ((64 * i) << a.page_shift));
-      vexp = v_exps[(uint64_t)page * a.exp_page_stride];
     };
-    int e_ref = 0;                                  // the exponent that O is held at once the staged tile is added
-    float e_drop = 1.0f;                            // and what O is multiplied by before that
-    uint32_t block_ok = 0;                          // bit b: the tile's 16-key block b has a page
+    // (ONE: once every piece of the tile before is converted, since they share the exponent)
+    auto load_k_exp = [&] {
+      if constexpr (ONE) {
+        const uint32_t page = (uint32_t)kid[0] < a.pages ? kid[0] : 0;
+        kexp[0] = scalar_byte(k_exps + (uint64_t)page * a.exp_page_stride);
+      }
+    };
+    auto load_v = [&](int t, int i) {
+      const int base = key_of(t), block = ONE ? 0 : 16 * (tid & 3);
+      const bool ok = ((uint32_t)vid < a.pages) & (base + block < en.end);
+      const uint32_t page = ok ? vid : 0;
+      if (i == 0) {
+        vok = ok;
+        if constexpr (ONE) vexp = scalar_byte(v_exps + (uint64_t)page * a.exp_page_stride);
+        else vexp = v_exps[(uint64_t)page * a.exp_page_stride];
+      }
+      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride + (uint32_t)((base + block) & page_mask);
+      const uint32_t off = (uint32_t)(((tid >> 2) + 64 * i) << a.page_shift) + (ONE ? 16 * (tid & 3) : 0);
+      vw[i] = *reinterpret_cast<const uint4*>(vp + off);
+    };
     auto whole_tile = [&](int base) {
       return base + kTile - 1 <= p_lo && base + kTile <= en.end &&
              (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks);
     };
-    auto stage = [&](int t, int buf, int flag) {
+    int e_ref = 0;                                  // the exponent that O is held at once the staged tile is added
+    float e_drop = 1.0f;                            // and what O is multiplied by before that
+    float v_scale = 1.0f;
+    uint32_t block_ok = 0;                          // bit b: the staged V tile's 16-key block b has a page
+    // before V of tile t is converted into stage buf: hidden values out of the way, and its scale
+    auto prepare_v = [&](int t, int buf) {
       const int base = key_of(t);
-      const uint32_t ok4 = (uint32_t)__ballot(vok) & 15u;
-      block_ok = ok4;
-      uint8_t* sk = s_stage + buf * (G::kStageK + G::kStageV);
-      uint8_t* sv = sk + G::kStageK;
+      block_ok = ONE ? (vok ? 15u : 0u) : (uint32_t)__ballot(vok) & 15u;
       int ev = vexp;
-      if (!whole_tile(base) || ok4 != 15u) {
+      if (!whole_tile(base) || block_ok != 15u) {
         // values of keys that no row sees may be anything, NaN included: zero them
         const int j0 = base + 16 * (tid & 3);
         const Sight widest = sight_of(a, p_hi, p_lo, en.end, j0), least = sight_of(a, p_lo, p_hi, en.end, j0);
@@ -1085,35 +1136,46 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
           vw[i].y &= byte_mask(any >> 4);
           vw[i].z &= byte_mask(any >> 8);
           vw[i].w &= byte_mask(any >> 12);
-          // such a NaN leaves the product; the outputs that it reaches become NaN at the end
+          // a NaN that some rows see and others do not leaves the product; the outputs that it reaches become NaN at the
+          // end
           const uint32_t found = take_nan(vw[i], some);
           s_where[buf][(tid >> 2) + 64 * i][tid & 3] = (uint16_t)found;
           nan |= found;
         }
-        if (nan) s_nan[flag] = 1;
+        if (nan) s_nan[t % 3] = 1;
       }
       int e_max = max(ev, 0);
-      e_max = max(e_max, __shfl_xor(e_max, 1));
-      e_max = max(e_max, __shfl_xor(e_max, 2));
+      if (!ONE || block_ok == 0 || !whole_tile(base)) {
+        e_max = max(e_max, __shfl_xor(e_max, 1));
+        e_max = max(e_max, __shfl_xor(e_max, 2));
+      }
+      e_max = __builtin_amdgcn_readfirstlane(e_max);
       const int e_new = max(e_ref, e_max);
       e_drop = exp_bits(127 + max(e_ref - e_new, -126));
       e_ref = e_new;
-      const float vs = exp_bits(127 + max(ev - e_ref, -126));
-#pragma unroll
-      for (int i = 0; i < G::kLoads; ++i) {
-        const int piece = tid + 256 * i, row = key_row(piece / (D / 16)), unit = piece % (D / 16) * 2;
-        const float ks = exp_bits(kexp[i]);
-        uint8_t* dst = sk + row * D * 2;
-        *reinterpret_cast<bf16x8_t*>(dst + ((unit ^ (row & 7)) * 16)) = e4m3x8_to_bf16(kw[i].x, kw[i].y, ks);
-        *reinterpret_cast<bf16x8_t*>(dst + (((unit + 1) ^ (row & 7)) * 16)) = e4m3x8_to_bf16(kw[i].z, kw[i].w, ks);
-        const int dim = (tid >> 2) + 64 * i, vu = (tid & 3) * 2;
-        uint8_t* vdst = sv + dim * kTile * 2;
-        *reinterpret_cast<half8_t*>(vdst + ((vu ^ (dim & 7)) * 16)) = e4m3x8_to_f16(vw[i].x, vw[i].y, vs);
-        *reinterpret_cast<half8_t*>(vdst + (((vu + 1) ^ (dim & 7)) * 16)) = e4m3x8_to_f16(vw[i].z, vw[i].w, vs);
-      }
+      v_scale = exp_bits(127 + max(ev - e_ref, -126));
+    };
+    auto convert_k = [&](int i, int buf) {
+      const int piece = tid + 256 * i, row = key_row(piece / (D / 16)), unit = piece % (D / 16) * 2;
+      const float ks = exp_bits(kexp[ONE ? 0 : i]);
+      uint8_t* dst = s_k + buf * G::kStageK + row * G::kRowK + unit * 16;
+      *reinterpret_cast<bf16x8_t*>(dst) = e4m3x8_to_bf16(kw[i].x, kw[i].y, ks);
+      *reinterpret_cast<bf16x8_t*>(dst + 16) = e4m3x8_to_bf16(kw[i].z, kw[i].w, ks);
+    };
+    auto convert_v = [&](int i, int buf) {
+      const int dim = (tid >> 2) + 64 * i, vu = (tid & 3) * 2;
+      uint8_t* dst = s_v + buf * G::kStageV + dim * G::kRowV + vu * 16;
+      *reinterpret_cast<half8_t*>(dst) = e4m3x8_to_f16(vw[i].x, vw[i].y, v_scale);
+      *reinterpret_cast<half8_t*>(dst + 16) = e4m3x8_to_f16(vw[i].z, vw[i].w, v_scale);
+    };
+    auto read_k = [&](int buf, int x, int kb) {
+      return *reinterpret_cast<const bf16x8_t*>(s_k + buf * G::kStageK + (32 * kb + c) * G::kRowK + (2 * x + hf) * 16);
+    };
+    auto read_v = [&](int buf, int u, int dt) {
+      return *reinterpret_cast<const half8_t*>(s_v + buf * G::kStageV + (32 * dt + c) * G::kRowV + (2 * u + hf) * 16);
     };
 
-    float16_t acc[G::kDT];
+    float16_t acc[G::kDT], s[2];
     float m_run = -__builtin_inff(), l_run = 0.0f;
     uint32_t poison[D / 64] = {};         // outputs that a NaN reached which not every row sees: bit 16 dt + 4 a + i
 #pragma unroll
@@ -1124,105 +1186,176 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     __syncthreads();        // the stages' and flags' earlier readers are done
     if (tid < 3) s_nan[tid] = 0;
     __syncthreads();
-    pages_at(t0);
-    load(t0);
-    if (t0 + 1 < t1) pages_at(t0 + 1);
-    stage(t0, 0, 0);
+    // tiles are numbered from 0 within the run for their buffers (t - t0), and from t0 for their keys
+    k_page(t0);
+    v_page(t0);
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      load_k(t0, i);
+      load_v(t0, i);
+    }
+    load_k_exp();
+    k_page(t0 + 1);
+    v_page(t0 + 1);
+    prepare_v(t0, t0 & 1);
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      convert_k(i, t0 & 1);
+      convert_v(i, t0 & 1);
+    }
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      load_k(t0 + 1, i);
+      load_v(t0 + 1, i);
+    }
+    load_k_exp();
+    k_page(t0 + 2);
+    v_page(t0 + 2);
+    float drop = e_drop;                // of the tile whose PV comes next
+    uint32_t tile_ok = block_ok;
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      convert_k(i, (t0 + 1) & 1);
+      load_k(t0 + 2, i);
+    }
+    load_k_exp();
+    k_page(t0 + 3);
     __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_k(t0 & 1, x, kb), qb[x], s[kb], 0, 0, 0);
+    }
+    __syncthreads();                    // K of the first tile is read before the step converts the third into its place
+
     for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      const bool more = t + 1 < t1;
-      const float drop = e_drop;
-      const uint32_t tile_ok = block_ok;
-      if (more) load(t + 1);
-      if (t + 2 < t1) pages_at(t + 2);
-      const int slot = (t - t0) % 3;
-      if (wave_live) {
-        const int base = key_of(t);
-        const uint8_t* sk = s_stage + buf * (G::kStageK + G::kStageV);
-        const uint8_t* sv = sk + G::kStageK;
-        float16_t s[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
-          const uint8_t* row = sk + (32 * kb + c) * D * 2;
-#pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            const bf16x8_t k = *reinterpret_cast<const bf16x8_t*>(row + (((2 * x + hf) ^ (c & 7)) * 16));
-            s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qb[x], s[kb], 0, 0, 0);
-          }
-        }
-        // s[kb][4 a + i] is key base + 32 kb + 16 (a / 2) + 8 hf + 4 (a % 2) + i
-        const bool whole = whole_tile(base) && tile_ok == 15u;
-        uint32_t vis = 0xFFFFFFFFu;
-        if (!whole) {
-          vis = 0;
-          const Sight sight = sight_of(a, pos, pos, en.end, base + 8 * hf);
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int in_tile = 32 * kb + 16 * (i >> 3) + (i & 7);
-              const bool see = sight.sees(in_tile) & ((tile_ok >> (in_tile >> 4) & 1u) != 0);
-              vis |= see ? 1u << (16 * kb + i) : 0u;
-              s[kb][i] = see ? s[kb][i] : -__builtin_inff();
-            }
-        }
-        float mx = -__builtin_inff();
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-        {
-          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-          mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale;
-        }
-        const float m_new = fmaxf(m_run, mx);
-        const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
-        m_run = m_new;
-        half8_t pb[4];
-        float sum = 0.0f;
+      const int now = t & 1, other = now ^ 1;
+      const int base = key_of(t);
+      // s[kb][4 a + i] is key base + 32 kb + 16 (a / 2) + 8 hf + 4 (a % 2) + i
+      uint32_t vis = 0xFFFFFFFFu;
+      if (!whole_tile(base) || tile_ok != 15u) {
+        vis = 0;
+        const Sight sight = sight_of(a, pos, pos, en.end, base + 8 * hf);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.scale, -mu));
-            sum += p;
-            pb[2 * kb + (i >> 3)][i & 7] = (_Float16)p;
-          }
-        l_run = l_run * alpha + sum;
-        const float f = alpha * drop;
-        if (__ballot(f != 1.0f)) {
-#pragma unroll
-          for (int dt = 0; dt < G::kDT; ++dt) acc[dt] *= f;
-        }
-        if (s_nan[slot]) {      // (never in a whole tile: its map is written only beside the flag)
-          // vis holds keys 16 u + 8 hf + i as bit 8 u + i: the row's 16-bit blocks are its bytes and the other half's
-          const auto sw = __builtin_amdgcn_permlane32_swap(vis, vis, false, false);
-          const uint32_t low = sw[0], high = sw[1];
-#pragma unroll 1
-          for (int k = 0; k < D / 2; ++k) {          // acc[k / 16][4 a + i]: dimension 32 (k / 16) + 8 a + 4 hf + i
-            const uint16_t* w = s_where[buf][32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hf + (k & 3)];
-            uint32_t hit = 0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) hit |= w[u] & ((low >> (8 * u) & 0xFFu) | (high >> (8 * u) & 0xFFu) << 8);
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) poison[x] |= hit && k >> 5 == x ? 1u << (k & 31) : 0u;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int dt = 0; dt < G::kDT; ++dt) {
-            const half8_t v = *reinterpret_cast<const half8_t*>(sv + (32 * dt + c) * kTile * 2 +
-                                                                (((2 * u + hf) ^ (c & 7)) * 16));
-            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pb[u], acc[dt], 0, 0, 0);
+            const int in_tile = 32 * kb + 16 * (i >> 3) + (i & 7);
+            const bool see = sight.sees(in_tile) & ((tile_ok >> (in_tile >> 4) & 1u) != 0);
+            vis |= see ? 1u << (16 * kb + i) : 0u;
+            s[kb][i] = see ? s[kb][i] : -__builtin_inff();
           }
       }
-      if (more) stage(t + 1, buf ^ 1, (t + 1 - t0) % 3);
-      if (tid == 0) s_nan[(t + 2 - t0) % 3] = 0;      // read last in the step before this one
+      // scores of the next tile beside this one's softmax: a quarter of the chunks for the maximum, the others for the
+      // exponentials
+      float16_t n[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) n[kb][i] = 0.0f;
+      xt_u32x4_t pw[4];
+      float mx = -__builtin_inff(), mu = 0.0f, alpha = 1.0f, sum = 0.0f;
+      constexpr int kMaxChunks = NX / 4;
+      bf16x8_t kf[2][2];
+      kf[0][0] = read_k(other, 0, 0);
+      kf[0][1] = read_k(other, 0, 1);
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        if (x + 1 < NX) {
+          kf[(x + 1) & 1][0] = read_k(other, x + 1, 0);
+          kf[(x + 1) & 1][1] = read_k(other, x + 1, 1);
+        }
+        n[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[x & 1][0], qb[x], n[0], 0, 0, 0);
+        n[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[x & 1][1], qb[x], n[1], 0, 0, 0);
+        if (x < kMaxChunks) {
+          constexpr int kEach = 32 / kMaxChunks;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) mx = fmaxf(mx, s[(x * kEach + e) >> 4][(x * kEach + e) & 15]);
+          if (x == kMaxChunks - 1) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale;
+            const float m_new = fmaxf(m_run, mx);
+            mu = m_new == -__builtin_inff() ? 0.0f : m_new;
+            alpha = __builtin_amdgcn_exp2f(m_run - mu);
+            m_run = m_new;
+          }
+        } else {
+          constexpr int kLeft = NX - kMaxChunks;
+          const int y = x - kMaxChunks, from = 16 * y / kLeft * 2, to = 16 * (y + 1) / kLeft * 2;   // pairs
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            if (e >= from && e < to) {
+              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 4][e & 15], a.scale, -mu));
+              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 4][(e & 15) + 1], a.scale, -mu));
+              sum += p0 + p1;
+              uint32_t pair = pack2_16<false>(p0, p1);
+              keep_here(pair);
+              pw[e >> 3][(e & 7) / 2] = pair;
+            }
+          keep_here(sum);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      l_run = l_run * alpha + sum;
+      if (s_nan[t % 3]) {      // (never in a whole tile: its map is written only beside the flag)
+        // vis holds keys 16 u + 8 hf + i as bit 8 u + i: the row's 16-bit blocks are its bytes and the other half's
+        const auto sw = __builtin_amdgcn_permlane32_swap(vis, vis, false, false);
+        const uint32_t low = sw[0], high = sw[1];
+#pragma unroll 1
+        for (int k = 0; k < D / 2; ++k) {          // acc[k / 16][4 a + i]: dimension 32 (k / 16) + 8 a + 4 hf + i
+          const uint16_t* w = s_where[now][32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hf + (k & 3)];
+          uint32_t hit = 0;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) hit |= w[u] & ((low >> (8 * u) & 0xFFu) | (high >> (8 * u) & 0xFFu) << 8);
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) poison[x] |= hit && k >> 5 == x ? 1u << (k & 31) : 0u;
+        }
+      }
+      const float f = alpha * drop;
+      if (__ballot(f != 1.0f)) {
+#pragma unroll
+        for (int dt = 0; dt < G::kDT; ++dt) acc[dt] *= f;
+      }
+      prepare_v(t + 1, other);
+      drop = e_drop;
+      tile_ok = block_ok;
+      // this tile's values beside the conversion of the next V and the K after it, each register refilled once it is
+      // converted
+      half8_t vf[2][G::kDT];
+#pragma unroll
+      for (int dt = 0; dt < G::kDT; ++dt) vf[0][dt] = read_v(now, 0, dt);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (u + 1 < 4) {
+#pragma unroll
+          for (int dt = 0; dt < G::kDT; ++dt) vf[(u + 1) & 1][dt] = read_v(now, u + 1, dt);
+        }
+#pragma unroll
+        for (int dt = 0; dt < G::kDT; ++dt)
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[u & 1][dt], __builtin_bit_cast(half8_t, pw[u]), acc[dt],
+                                                           0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < G::kLoads; ++i) {
+          if (2 * i * 4 / (2 * G::kLoads) == u) {
+            convert_v(i, other);
+            load_v(t + 2, i);
+          }
+          if ((2 * i + 1) * 4 / (2 * G::kLoads) == u) {
+            convert_k(i, now);
+            load_k(t + 3, i);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      load_k_exp();
+      v_page(t + 3);
+      k_page(t + 4);
+      if (tid == 0) s_nan[(t + 2) % 3] = 0;      // read last in the step before this one
+      s[0] = n[0];
+      s[1] = n[1];
       __syncthreads();
     }
 
@@ -1395,12 +1528,18 @@ static int launch_decode(const char* what, const AttnArgs& a, int groups, xt_str
   return check_launch(what);
 }
 
+template <int D, bool ONE>
+static int launch_prefill_as(const char* what, const AttnArgs& a, int groups, xt_stream_t stream) {
+  const size_t lds = PrefillGeo<D>::kLds;
+  if (const int st = allow_lds((const void*)prefill_kernel<D, ONE>, lds, what)) return st;
+  prefill_kernel<D, ONE><<<groups, 256, lds, stream>>>(a);
+  return check_launch(what);
+}
+
 template <int D>
 static int launch_prefill(const char* what, const AttnArgs& a, int groups, xt_stream_t stream) {
-  const size_t lds = PrefillGeo<D>::kLds;
-  if (const int st = allow_lds((const void*)prefill_kernel<D>, lds, what)) return st;
-  prefill_kernel<D><<<groups, 256, lds, stream>>>(a);
-  return check_launch(what);
+  return 1 << a.page_shift >= kTile ? launch_prefill_as<D, true>(what, a, groups, stream)
+                                    : launch_prefill_as<D, false>(what, a, groups, stream);
 }
 
 extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
