@@ -12,6 +12,8 @@
 // less than one binade of range, while a power of two makes every step but the rounding to E4M3 exact: a page whose
 // scale grows keeps its normal values unchanged, and a K value with its scale is a BF16 value, so the first product takes
 // the BF16 query and the keys exactly.
+#include <type_traits>
+
 #include "xt_common.h"
 #include "xt_host.h"
 
@@ -952,19 +954,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
 
 // --- attention: many rows per request -----------------------------------------------------------------------------------
 
-// 128 query rows a workgroup, 32 for each of its 4 waves, on 32x32 MFMAs. The workgroup dequantizes each 64-key tile
+// 32 W query rows a workgroup, 32 for each of its W waves, on 32x32 MFMAs. The workgroup dequantizes each 64-key tile
 // once, K to BF16 and V to FP16, into one of two LDS stages while it computes on the other: a wave's 32 rows alone would
-// pay the conversion four times over. K rows lie in LDS in the order of the A rows of S^T (key_row).
-template <int D>
+// pay the conversion W times over. K rows lie in LDS in the order of the A rows of S^T (key_row).
+template <int D, int W>
 struct PrefillGeo {
-  static constexpr int kM = 128;
+  static constexpr int kM = 32 * W, kThreads = 64 * W;
   // Rows of a stage are padded by 16 bytes: LDS reads 16 lanes' 16-byte units at a time from 64 banks, and 16 rows in a
   // row, an odd number of units apart, put the same unit at 16 different places. (An XOR of the unit with the row
   // saves the padding, but costs an address register or instruction for every unit of a row.)
   static constexpr int kRowK = D * 2 + 16, kRowV = kTile * 2 + 16;
   static constexpr int kStageK = kTile * kRowK, kStageV = D * kRowV;
   static constexpr int kLds = 2 * (kStageK + kStageV);
-  static constexpr int kLoads = kTile * D / 16 / 256;    // 16-byte pieces of K, and of V, that a thread stages: D / 64
+  static constexpr int kLoads = kTile * D / 16 / kThreads;    // 16-byte pieces of K, and of V, that a thread stages
   static constexpr int kDT = D / 32;
 };
 
@@ -986,29 +988,32 @@ __device__ inline void keep_here(T& x) {
 }
 
 // The step of tile t: S(t + 1) = K(t + 1) Q^T beside the softmax of S(t), then O += V(t) P(t) beside the conversion of
-// K(t + 2) and V(t + 1), which lie in registers, and the loads of the pair after them. MFMAs and vector instructions of
+// V(t + 1) and K(t + 2), which lie in registers, and the loads of the pair after them. MFMAs and vector instructions of
 // one wave alternate, because two waves on a SIMD (what 256 registers allow) do not fill it otherwise: a wave issues an
-// instruction every 8 clocks at most, a vector instruction takes 4 and an MFMA 32. Fences to the scheduler keep that order.
+// instruction every 8 clocks at most, of any kind, while a vector instruction takes 4 and an MFMA 32. Fences to the
+// scheduler keep that order; for the same reason the step is kept short of scalar work, and written out twice so that
+// stages have fixed addresses and scores need no copies.
 //
 // ONE: pages of 64 tokens and more, so that a tile lies in one page, whose address is then a scalar.
-template <int D, bool ONE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs a) {
+template <int D, int W, bool ONE>
+__global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using G = PrefillGeo<D>;
-  constexpr int M = G::kM, kPitch = D + 4, kSlot = M * kPitch, NX = D / 16;
+  using G = PrefillGeo<D, W>;
+  constexpr int M = G::kM, T = G::kThreads, kPitch = D + 4, kSlot = M * kPitch, NX = D / 16, L = G::kLoads;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_stage[];   // (ds_read_b128 off 16 bytes takes thrice as long)
   __shared__ int s_last;
-  // whether a stage's V holds a NaN that some rows see and others do not, and where: [stage][dim][4 blocks of 16 keys]
-  __shared__ int s_nan[3];
+  // whether a tile's V holds a NaN that some rows see and others do not (of four tiles), and where: [stage][dim][4 blocks
+  // of 16 keys]
+  __shared__ int s_nan[4];
   __shared__ __attribute__((aligned(16))) uint16_t s_where[2][D][4];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
   const int groups = (int)gridDim.x;
   const int wg = xcd_order((int)blockIdx.x, groups);
-  Share sh = share_of<256>(a, M, groups, wg);
+  Share sh = share_of<T>(a, M, groups, wg);
   const int page_mask = (1 << a.page_shift) - 1;
-  uint8_t* const s_k = s_stage;                       // [2][64 keys][D] BF16
-  uint8_t* const s_v = s_stage + 2 * G::kStageK;      // [2][D][64 keys] FP16
+  uint8_t* const s_k = s_stage;                       // [2][64 keys] rows of D BF16
+  uint8_t* const s_v = s_stage + 2 * G::kStageK;      // [2][D] rows of 64 keys, FP16
 
   while (sh.pos < sh.end) {
     const Entry en = entry_at(a, sh.entry, M);
@@ -1035,77 +1040,84 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
       }
     }
     const int p_lo = en.start + en.r0 / a.group, p_hi = en.start + (en.r1 - 1) / a.group;
-    // (tiles past the run repeat its last one: the step loads and multiplies ahead without asking)
-    auto key_of = [&](int t) {
-      const int u = min(t, t1 - 1);
-      return kTile * (u < en.sink_tiles ? u : u + en.skip);
+    auto key_of = [&](int t) { return kTile * (t < en.sink_tiles ? t : t + en.skip); };
+    // the tiles that every row sees whole: t < whole_hi and (t >= whole_lo or t < whole_sink)
+    const int whole_hi = (p_lo < 0 ? 0 : min(p_lo + 1, en.end) / kTile) - (en.skip > 0 ? en.skip : 0);
+    int whole_lo = 0, whole_sink = 0;
+    if (a.window > 0) {
+      const int from = p_hi - a.window + 1;               // keys from here on are in every row's window
+      whole_lo = from > 0 ? (from + kTile - 1) / kTile - en.skip : 0;
+      whole_sink = min(a.sinks / kTile, en.sink_tiles);
+    }
+    auto whole_tile = [&](int t) {
+      // (with skipped tiles the sink tiles lie whole below every row)
+      return (t < whole_hi || (en.skip > 0 && t < whole_sink)) && (t >= whole_lo || t < whole_sink);
     };
 
-    // staging: thread tid holds pieces tid + 256 i of the K block (key = piece / (D / 16)) and of the V block (dimension
-    // = piece / 4, 16 keys piece % 4)
+    // staging: thread tid holds pieces tid + T i of the K block (key = piece / (D / 16)) and of the V block (dimension =
+    // piece / 4, 16 keys piece % 4). The K of a tile is loaded a step before its V, from the page that `next` found
+    // a step earlier still.
     const int32_t* row_table = a.table + (int64_t)en.b * a.table_stride;
     const uint8_t *k_base = a.kp + head * a.head_stride, *v_base = a.vp + head * a.head_stride;
     const uint8_t *k_exps = a.ke + head * a.exp_head_stride, *v_exps = a.ve + head * a.exp_head_stride;
     const int last = max(en.end - 1, 0);            // keys past it look its page up, and are masked
-    uint4 kw[G::kLoads], vw[G::kLoads];
-    int kid[ONE ? 1 : G::kLoads], vid = 0;          // pages of the tiles to load next
-    int kexp[ONE ? 1 : G::kLoads], vexp = 0;        // exponents of the tiles to stage
-    bool vok = false;                               // whether the V block holds anything
-    auto k_page = [&](int t) {
+    struct Tile {
+      int base;                                     // first key
+      int k[ONE ? 1 : L], v;                        // pages of this thread's pieces
+    };
+    Tile next;
+    auto find = [&](int t) {                        // (tiles past the run repeat its last one)
+      Tile x;
+      x.base = key_of(min(t, t1 - 1));
       if constexpr (ONE) {
-        kid[0] = uniform_load(row_table + (min(key_of(t), last) >> a.page_shift));
+        x.k[0] = x.v = uniform_load(row_table + (min(x.base, last) >> a.page_shift));
       } else {
 #pragma unroll
-        for (int i = 0; i < G::kLoads; ++i)
-          kid[i] = row_table[min(key_of(t) + (tid + 256 * i) / (D / 16), last) >> a.page_shift];
+        for (int i = 0; i < L; ++i) x.k[i] = row_table[min(x.base + (tid + T * i) / (D / 16), last) >> a.page_shift];
+        x.v = row_table[min(x.base + 16 * (tid & 3), last) >> a.page_shift];
       }
+      return x;
     };
-    auto v_page = [&](int t) {
-      if constexpr (ONE) vid = uniform_load(row_table + (min(key_of(t), last) >> a.page_shift));
-      else vid = row_table[min(key_of(t) + 16 * (tid & 3), last) >> a.page_shift];
-    };
+    uint4 kw[L], vw[L];
+    int kexp[ONE ? 1 : L], vexp = 0;                // exponents of the tiles to stage
+    bool vok = false;                               // whether the V block holds anything
     // one byte by a scalar load of the word that holds it
     auto scalar_byte = [](const uint8_t* p) {
       const uint64_t at = (uint64_t)p;
       return uniform_load(reinterpret_cast<const int32_t*>(at & ~(uint64_t)3)) >> (8 * (int)(at & 3)) & 0xFF;
     };
-    auto load_k = [&](int t, int i) {
-      const int base = key_of(t);
-      const int32_t id = kid[ONE ? 0 : i];
+    auto load_k = [&](const Tile& x, int i) {
+      const int32_t id = x.k[ONE ? 0 : i];
       const uint32_t page = (uint32_t)id < a.pages ? id : 0;
       if constexpr (ONE) {
-        const uint8_t* block = k_base + (uint64_t)page * a.page_stride + (uint32_t)((base & page_mask) * D);
-        kw[i] = *reinterpret_cast<const uint4*>(block + (uint32_t)(tid * 16) + 4096 * i);
+        const uint8_t* block = k_base + (uint64_t)page * a.page_stride + (uint32_t)((x.base & page_mask) * D);
+        kw[i] = *reinterpret_cast<const uint4*>(block + (uint32_t)(tid * 16) + 16 * T * i);
       } else {
-        const int piece = tid + 256 * i;
+        const int piece = tid + T * i;
         kw[i] = *reinterpret_cast<const uint4*>(k_base + (uint64_t)page * a.page_stride +
-                                                (((base + piece / (D / 16)) & page_mask) * D + piece % (D / 16) * 16));
+                                                (((x.base + piece / (D / 16)) & page_mask) * D + piece % (D / 16) * 16));
         kexp[i] = k_exps[(uint64_t)page * a.exp_page_stride];
       }
     };
     // (ONE: once every piece of the tile before is converted, since they share the exponent)
-    auto load_k_exp = [&] {
+    auto load_k_exp = [&](const Tile& x) {
       if constexpr (ONE) {
-        const uint32_t page = (uint32_t)kid[0] < a.pages ? kid[0] : 0;
+        const uint32_t page = (uint32_t)x.k[0] < a.pages ? x.k[0] : 0;
         kexp[0] = scalar_byte(k_exps + (uint64_t)page * a.exp_page_stride);
       }
     };
-    auto load_v = [&](int t, int i) {
-      const int base = key_of(t), block = ONE ? 0 : 16 * (tid & 3);
-      const bool ok = ((uint32_t)vid < a.pages) & (base + block < en.end);
-      const uint32_t page = ok ? vid : 0;
+    const uint32_t v_off = (uint32_t)((tid >> 2) << a.page_shift) + (ONE ? 16 * (tid & 3) : 0);
+    auto load_v = [&](const Tile& x, int i) {
+      const int block = ONE ? 0 : 16 * (tid & 3);
+      const bool ok = ((uint32_t)x.v < a.pages) & (x.base + block < en.end);
+      const uint32_t page = ok ? x.v : 0;
       if (i == 0) {
         vok = ok;
         if constexpr (ONE) vexp = scalar_byte(v_exps + (uint64_t)page * a.exp_page_stride);
         else vexp = v_exps[(uint64_t)page * a.exp_page_stride];
       }
-      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride + (uint32_t)((base + block) & page_mask);
-      const uint32_t off = (uint32_t)(((tid >> 2) + 64 * i) << a.page_shift) + (ONE ? 16 * (tid & 3) : 0);
-      vw[i] = *reinterpret_cast<const uint4*>(vp + off);
-    };
-    auto whole_tile = [&](int base) {
-      return base + kTile - 1 <= p_lo && base + kTile <= en.end &&
-             (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks);
+      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride + (uint32_t)((x.base + block) & page_mask);
+      vw[i] = *reinterpret_cast<const uint4*>(vp + ((uint32_t)(16 * W * i) << a.page_shift) + v_off);
     };
     int e_ref = 0;                                  // the exponent that O is held at once the staged tile is added
     float e_drop = 1.0f;                            // and what O is multiplied by before that
@@ -1113,12 +1125,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     uint32_t block_ok = 0;                          // bit b: the staged V tile's 16-key block b has a page
     // before V of tile t is converted into stage buf: hidden values out of the way, and its scale
     auto prepare_v = [&](int t, int buf) {
-      const int base = key_of(t);
       block_ok = ONE ? (vok ? 15u : 0u) : (uint32_t)__ballot(vok) & 15u;
+      const bool plain = whole_tile(t) && t < t1 && block_ok == 15u;
       int ev = vexp;
-      if (!whole_tile(base) || block_ok != 15u) {
+      if (!plain) {
         // values of keys that no row sees may be anything, NaN included: zero them
-        const int j0 = base + 16 * (tid & 3);
+        const int j0 = key_of(min(t, t1 - 1)) + 16 * (tid & 3);
         const Sight widest = sight_of(a, p_hi, p_lo, en.end, j0), least = sight_of(a, p_lo, p_hi, en.end, j0);
         uint32_t any = 0, all = 0;
 #pragma unroll
@@ -1131,7 +1143,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
         const uint32_t some = any & ~all;
         uint32_t nan = 0;
 #pragma unroll
-        for (int i = 0; i < G::kLoads; ++i) {
+        for (int i = 0; i < L; ++i) {
           vw[i].x &= byte_mask(any);
           vw[i].y &= byte_mask(any >> 4);
           vw[i].z &= byte_mask(any >> 8);
@@ -1139,43 +1151,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
           // a NaN that some rows see and others do not leaves the product; the outputs that it reaches become NaN at the
           // end
           const uint32_t found = take_nan(vw[i], some);
-          s_where[buf][(tid >> 2) + 64 * i][tid & 3] = (uint16_t)found;
+          s_where[buf][(tid >> 2) + 16 * W * i][tid & 3] = (uint16_t)found;
           nan |= found;
         }
-        if (nan) s_nan[t % 3] = 1;
+        if (nan) s_nan[t & 3] = 1;
       }
       int e_max = max(ev, 0);
-      if (!ONE || block_ok == 0 || !whole_tile(base)) {
+      if (!ONE || !plain) {
         e_max = max(e_max, __shfl_xor(e_max, 1));
         e_max = max(e_max, __shfl_xor(e_max, 2));
+        e_max = __builtin_amdgcn_readfirstlane(e_max);
       }
-      e_max = __builtin_amdgcn_readfirstlane(e_max);
       const int e_new = max(e_ref, e_max);
       e_drop = exp_bits(127 + max(e_ref - e_new, -126));
       e_ref = e_new;
       v_scale = exp_bits(127 + max(ev - e_ref, -126));
     };
+    // (the LDS places of a thread's first pieces; the others are a fixed number of rows further)
+    const int k_put = key_row(tid / (D / 16)) * G::kRowK + tid % (D / 16) * 32;
+    const int v_put = (tid >> 2) * G::kRowV + (tid & 3) * 32;
     auto convert_k = [&](int i, int buf) {
-      const int piece = tid + 256 * i, row = key_row(piece / (D / 16)), unit = piece % (D / 16) * 2;
+      constexpr int kRows = T / (D / 16);           // keys between a thread's pieces: their LDS rows differ as they do
       const float ks = exp_bits(kexp[ONE ? 0 : i]);
-      uint8_t* dst = s_k + buf * G::kStageK + row * G::kRowK + unit * 16;
+      const int put = kRows % 16 == 0 ? k_put + kRows * i * G::kRowK
+                                      : key_row((tid + T * i) / (D / 16)) * G::kRowK + tid % (D / 16) * 32;
+      uint8_t* dst = s_k + buf * G::kStageK + put;
       *reinterpret_cast<bf16x8_t*>(dst) = e4m3x8_to_bf16(kw[i].x, kw[i].y, ks);
       *reinterpret_cast<bf16x8_t*>(dst + 16) = e4m3x8_to_bf16(kw[i].z, kw[i].w, ks);
     };
     auto convert_v = [&](int i, int buf) {
-      const int dim = (tid >> 2) + 64 * i, vu = (tid & 3) * 2;
-      uint8_t* dst = s_v + buf * G::kStageV + dim * G::kRowV + vu * 16;
+      uint8_t* dst = s_v + buf * G::kStageV + v_put + 16 * W * i * G::kRowV;
       *reinterpret_cast<half8_t*>(dst) = e4m3x8_to_f16(vw[i].x, vw[i].y, v_scale);
       *reinterpret_cast<half8_t*>(dst + 16) = e4m3x8_to_f16(vw[i].z, vw[i].w, v_scale);
     };
+    const uint8_t *k_get = s_k + c * G::kRowK + hf * 16, *v_get = s_v + c * G::kRowV + hf * 16;
     auto read_k = [&](int buf, int x, int kb) {
-      return *reinterpret_cast<const bf16x8_t*>(s_k + buf * G::kStageK + (32 * kb + c) * G::kRowK + (2 * x + hf) * 16);
+      return *reinterpret_cast<const bf16x8_t*>(k_get + buf * G::kStageK + 32 * kb * G::kRowK + x * 32);
     };
     auto read_v = [&](int buf, int u, int dt) {
-      return *reinterpret_cast<const half8_t*>(s_v + buf * G::kStageV + (32 * dt + c) * G::kRowV + (2 * u + hf) * 16);
+      return *reinterpret_cast<const half8_t*>(v_get + buf * G::kStageV + 32 * dt * G::kRowV + u * 32);
     };
 
-    float16_t acc[G::kDT], s[2];
+    float16_t acc[G::kDT];
     float m_run = -__builtin_inff(), l_run = 0.0f;
     uint32_t poison[D / 64] = {};         // outputs that a NaN reached which not every row sees: bit 16 dt + 4 a + i
 #pragma unroll
@@ -1184,61 +1201,70 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
 
     __syncthreads();        // the stages' and flags' earlier readers are done
-    if (tid < 3) s_nan[tid] = 0;
+    if (tid < 4) s_nan[tid] = 0;
     __syncthreads();
-    // tiles are numbered from 0 within the run for their buffers (t - t0), and from t0 for their keys
-    k_page(t0);
-    v_page(t0);
+    // K and V of the first tile and K of the second into LDS, their successors into registers; the loads of all three on
+    // their way together
+    Tile now = find(t0);
+    next = find(t0 + 1);
+    const Tile third = find(t0 + 2);
 #pragma unroll
-    for (int i = 0; i < G::kLoads; ++i) {
-      load_k(t0, i);
-      load_v(t0, i);
+    for (int i = 0; i < L; ++i) {
+      load_k(now, i);
+      load_v(now, i);
     }
-    load_k_exp();
-    k_page(t0 + 1);
-    v_page(t0 + 1);
-    prepare_v(t0, t0 & 1);
+    load_k_exp(now);
+    uint4 k_first[L];
+    int e_first[ONE ? 1 : L];
 #pragma unroll
-    for (int i = 0; i < G::kLoads; ++i) {
-      convert_k(i, t0 & 1);
-      convert_v(i, t0 & 1);
+    for (int i = 0; i < L; ++i) {
+      k_first[i] = kw[i];
+      e_first[ONE ? 0 : i] = kexp[ONE ? 0 : i];
     }
 #pragma unroll
-    for (int i = 0; i < G::kLoads; ++i) {
-      load_k(t0 + 1, i);
-      load_v(t0 + 1, i);
-    }
-    load_k_exp();
-    k_page(t0 + 2);
-    v_page(t0 + 2);
+    for (int i = 0; i < L; ++i) load_k(next, i);
+    load_k_exp(next);
+    prepare_v(t0, 0);
+#pragma unroll
+    for (int i = 0; i < L; ++i) convert_v(i, 0);
+#pragma unroll
+    for (int i = 0; i < L; ++i) load_v(next, i);
     float drop = e_drop;                // of the tile whose PV comes next
     uint32_t tile_ok = block_ok;
 #pragma unroll
-    for (int i = 0; i < G::kLoads; ++i) {
-      convert_k(i, (t0 + 1) & 1);
-      load_k(t0 + 2, i);
+    for (int i = 0; i < L; ++i) convert_k(i, 1);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      kw[i] = k_first[i];
+      kexp[ONE ? 0 : i] = e_first[ONE ? 0 : i];
     }
-    load_k_exp();
-    k_page(t0 + 3);
+#pragma unroll
+    for (int i = 0; i < L; ++i) convert_k(i, 0);
+    now = third;
+#pragma unroll
+    for (int i = 0; i < L; ++i) load_k(now, i);
+    load_k_exp(now);
+    next = find(t0 + 3);                // in the step of t: `now` is tile t + 2, its K loaded; `next` t + 3
     __syncthreads();
+    float16_t s0[2], s1[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+      for (int i = 0; i < 16; ++i) s0[kb][i] = 0.0f;
 #pragma unroll
       for (int x = 0; x < NX; ++x)
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_k(t0 & 1, x, kb), qb[x], s[kb], 0, 0, 0);
+        s0[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_k(0, x, kb), qb[x], s0[kb], 0, 0, 0);
     }
     __syncthreads();                    // K of the first tile is read before the step converts the third into its place
 
-    for (int t = t0; t < t1; ++t) {
-      const int now = t & 1, other = now ^ 1;
-      const int base = key_of(t);
+    // s: this tile's scores, n: the next one's; B: this tile's stage
+    auto step = [&](int t, float16_t (&s)[2], float16_t (&n)[2], auto stage) {
+      constexpr int B = decltype(stage)::value;
       // s[kb][4 a + i] is key base + 32 kb + 16 (a / 2) + 8 hf + 4 (a % 2) + i
       uint32_t vis = 0xFFFFFFFFu;
-      if (!whole_tile(base) || tile_ok != 15u) {
+      if (!whole_tile(t) || tile_ok != 15u) {
         vis = 0;
-        const Sight sight = sight_of(a, pos, pos, en.end, base + 8 * hf);
+        const Sight sight = sight_of(a, pos, pos, en.end, key_of(t) + 8 * hf);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1251,7 +1277,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
       }
       // scores of the next tile beside this one's softmax: a quarter of the chunks for the maximum, the others for the
       // exponentials
-      float16_t n[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1260,13 +1285,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
       float mx = -__builtin_inff(), mu = 0.0f, alpha = 1.0f, sum = 0.0f;
       constexpr int kMaxChunks = NX / 4;
       bf16x8_t kf[2][2];
-      kf[0][0] = read_k(other, 0, 0);
-      kf[0][1] = read_k(other, 0, 1);
+      kf[0][0] = read_k(B ^ 1, 0, 0);
+      kf[0][1] = read_k(B ^ 1, 0, 1);
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
         if (x + 1 < NX) {
-          kf[(x + 1) & 1][0] = read_k(other, x + 1, 0);
-          kf[(x + 1) & 1][1] = read_k(other, x + 1, 1);
+          kf[(x + 1) & 1][0] = read_k(B ^ 1, x + 1, 0);
+          kf[(x + 1) & 1][1] = read_k(B ^ 1, x + 1, 1);
         }
         n[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[x & 1][0], qb[x], n[0], 0, 0, 0);
         n[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[x & 1][1], qb[x], n[1], 0, 0, 0);
@@ -1300,13 +1325,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
         __builtin_amdgcn_sched_barrier(0);
       }
       l_run = l_run * alpha + sum;
-      if (s_nan[t % 3]) {      // (never in a whole tile: its map is written only beside the flag)
+      if (!whole_tile(t) && s_nan[t & 3]) {
         // vis holds keys 16 u + 8 hf + i as bit 8 u + i: the row's 16-bit blocks are its bytes and the other half's
         const auto sw = __builtin_amdgcn_permlane32_swap(vis, vis, false, false);
         const uint32_t low = sw[0], high = sw[1];
 #pragma unroll 1
         for (int k = 0; k < D / 2; ++k) {          // acc[k / 16][4 a + i]: dimension 32 (k / 16) + 8 a + 4 hf + i
-          const uint16_t* w = s_where[now][32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hf + (k & 3)];
+          const uint16_t* w = s_where[B][32 * (k >> 4) + 8 * (k >> 2 & 3) + 4 * hf + (k & 3)];
           uint32_t hit = 0;
 #pragma unroll
           for (int u = 0; u < 4; ++u) hit |= w[u] & ((low >> (8 * u) & 0xFFu) | (high >> (8 * u) & 0xFFu) << 8);
@@ -1319,44 +1344,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
 #pragma unroll
         for (int dt = 0; dt < G::kDT; ++dt) acc[dt] *= f;
       }
-      prepare_v(t + 1, other);
+      prepare_v(t + 1, B ^ 1);
       drop = e_drop;
       tile_ok = block_ok;
       // this tile's values beside the conversion of the next V and the K after it, each register refilled once it is
       // converted
       half8_t vf[2][G::kDT];
 #pragma unroll
-      for (int dt = 0; dt < G::kDT; ++dt) vf[0][dt] = read_v(now, 0, dt);
+      for (int dt = 0; dt < G::kDT; ++dt) vf[0][dt] = read_v(B, 0, dt);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (u + 1 < 4) {
 #pragma unroll
-          for (int dt = 0; dt < G::kDT; ++dt) vf[(u + 1) & 1][dt] = read_v(now, u + 1, dt);
+          for (int dt = 0; dt < G::kDT; ++dt) vf[(u + 1) & 1][dt] = read_v(B, u + 1, dt);
         }
 #pragma unroll
         for (int dt = 0; dt < G::kDT; ++dt)
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[u & 1][dt], __builtin_bit_cast(half8_t, pw[u]), acc[dt],
                                                            0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < G::kLoads; ++i) {
-          if (2 * i * 4 / (2 * G::kLoads) == u) {
-            convert_v(i, other);
-            load_v(t + 2, i);
+        for (int i = 0; i < L; ++i) {
+          if (2 * i * 4 / (2 * L) == u) {
+            convert_v(i, B ^ 1);
+            load_v(now, i);
           }
-          if ((2 * i + 1) * 4 / (2 * G::kLoads) == u) {
-            convert_k(i, now);
-            load_k(t + 3, i);
+          if ((2 * i + 1) * 4 / (2 * L) == u) {
+            convert_k(i, B);
+            load_k(next, i);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      load_k_exp();
-      v_page(t + 3);
-      k_page(t + 4);
-      if (tid == 0) s_nan[(t + 2) % 3] = 0;      // read last in the step before this one
-      s[0] = n[0];
-      s[1] = n[1];
+      load_k_exp(next);
+      now = next;
+      next = find(t + 4);
+      if (tid == 0) s_nan[(t + 2) & 3] = 0;      // read last two steps ago
       __syncthreads();
+    };
+    for (int t = t0;;) {
+      step(t, s0, s1, std::integral_constant<int, 0>());
+      if (++t == t1) break;
+      step(t, s1, s0, std::integral_constant<int, 1>());
+      if (++t == t1) break;
     }
 
     // every wave has its rows whole: outputs or partials straight from registers (acc[dt][4 a + i] is dimension
@@ -1395,7 +1424,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(AttnArgs
     if (!alone) {
       int32_t* counter = a.counters + w_first;
       if (arrive_last(counter, w_last - w_first + 1, &s_last)) {
-        merge_partials<D, M, 256, 4, 4>(a, en, head, slot_of, w_first, w_last, pr);
+        merge_partials<D, M, T, 4, 4>(a, en, head, slot_of, w_first, w_last, pr);
         reset_counter(counter);
       }
     }
@@ -1409,11 +1438,14 @@ int page_shift_of(int page_size) {
                                                                                     : -1;
 }
 
+constexpr int64_t kWideRows = 256;       // rows of a request from which on 8 waves a workgroup win
 // Query rows of a workgroup, by the rows (tokens x heads of a group) that a request has on average: 16 or 32 in the
-// decode kernel, which reads its keys from memory wave by wave, else the prefill kernel's 128.
-int tile_rows(int64_t rows, int batch, int group) {
+// decode kernel, which reads its keys from memory wave by wave, else the prefill kernel's 32 for each wave: 4 waves, or 8
+// at head size 128 (at 64 a tile has too few pieces for 8 waves, at 256 a wave needs a SIMD's registers to itself).
+int tile_rows(int64_t rows, int batch, int group, int dim) {
   const int64_t all = rows * group;
-  return all <= 16 * (int64_t)batch ? 16 : all <= 32 * (int64_t)batch ? 32 : 128;
+  if (all <= 32 * (int64_t)batch) return all <= 16 * (int64_t)batch ? 16 : 32;
+  return dim == 128 && all > kWideRows * (int64_t)batch ? 256 : 128;
 }
 
 constexpr int64_t kMaxRows = 1 << 30;   // rows x heads of a group: 32-bit row numbers in the kernels
@@ -1424,19 +1456,20 @@ struct Launch {
   int partials;                // of m rows each
 };
 
-// Workgroups on the CUs at once: two of 4 waves to a CU. The prefill kernel has one workgroup to a slot, each with at
+// The prefill kernel has one workgroup to a slot, each with at
 // most two partials. The decode kernel has as many pieces as slots, or one for each (head, entry) and `sure` more a head
 // (piece_of); those with partials, of entries longer than a size that goes at most `room` times into their sum, are
 // fewer than twice that.
-Launch plan_launch(int rows, int batch, int heads, int group, bool ragged) {
+Launch plan_launch(int rows, int batch, int heads, int group, int dim, bool ragged) {
   Launch x;
-  x.m = tile_rows(rows, batch, group);
+  x.m = tile_rows(rows, batch, group, dim);
+  const bool prefill = x.m >= 128;
   x.entries = ragged ? (int)((int64_t)rows * group / x.m) + batch : batch * ((group + x.m - 1) / x.m);
-  x.slots = 2 * device_cus() / 8 * 8;
+  // 8 waves on a CU, but 4 of the prefill kernel at head size 256
+  x.slots = (x.m == 256 || (prefill && dim == 256) ? 1 : 2) * device_cus() / 8 * 8;
   const int64_t units = (int64_t)x.entries * heads, room = x.slots > heads ? x.slots : heads;
-  const int64_t most = x.m == 128 ? x.slots : units + room;
-  x.groups = (int)((most + 7) / 8 * 8);
-  x.partials = (int)(x.m == 128 ? 2 * x.slots : 2 * room);
+  x.groups = prefill ? x.slots : (int)((units + room + 7) / 8 * 8);
+  x.partials = (int)(prefill ? 2 * x.slots : 2 * room);
   return x;
 }
 
@@ -1513,8 +1546,8 @@ extern "C" size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_
   if (rows < 0 || batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || dim < 1 ||
       (int64_t)rows * (q_heads / kv_heads) > kMaxRows || (int64_t)batch * q_heads > kMaxRows)
     return 0;
-  const Launch x = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, true);
-  const Launch y = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, false);
+  const Launch x = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, dim, true);
+  const Launch y = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, dim, false);
   const size_t partial = (size_t)x.m * (dim + 4) * 4;
   const size_t a = counter_bytes(x) + x.partials * partial, b = counter_bytes(y) + y.partials * partial;
   return a > b ? a : b;
@@ -1528,18 +1561,18 @@ static int launch_decode(const char* what, const AttnArgs& a, int groups, xt_str
   return check_launch(what);
 }
 
-template <int D, bool ONE>
+template <int D, int W, bool ONE>
 static int launch_prefill_as(const char* what, const AttnArgs& a, int groups, xt_stream_t stream) {
-  const size_t lds = PrefillGeo<D>::kLds;
-  if (const int st = allow_lds((const void*)prefill_kernel<D, ONE>, lds, what)) return st;
-  prefill_kernel<D, ONE><<<groups, 256, lds, stream>>>(a);
+  const size_t lds = PrefillGeo<D, W>::kLds;
+  if (const int st = allow_lds((const void*)prefill_kernel<D, W, ONE>, lds, what)) return st;
+  prefill_kernel<D, W, ONE><<<groups, 64 * W, lds, stream>>>(a);
   return check_launch(what);
 }
 
-template <int D>
+template <int D, int W>
 static int launch_prefill(const char* what, const AttnArgs& a, int groups, xt_stream_t stream) {
-  return 1 << a.page_shift >= kTile ? launch_prefill_as<D, true>(what, a, groups, stream)
-                                    : launch_prefill_as<D, false>(what, a, groups, stream);
+  return 1 << a.page_shift >= kTile ? launch_prefill_as<D, W, true>(what, a, groups, stream)
+                                    : launch_prefill_as<D, W, false>(what, a, groups, stream);
 }
 
 extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
@@ -1572,7 +1605,7 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
   if (!q || !out || !aligned(q, 16) || q_row_stride % 8 || q_head_stride % 8 || !aligned(out, 8) ||
       out_row_stride % 4 || out_head_stride % 4)
     return fail(XT_EINVAL, "%s: query rows must be 16-byte aligned, output rows 8-byte aligned", what);
-  const Launch x = plan_launch(rows, batch, kv_heads, group, cu_q != nullptr);
+  const Launch x = plan_launch(rows, batch, kv_heads, group, dim, cu_q != nullptr);
   const int64_t tiles = ((int64_t)width * page_size + kTile - 1) / kTile;    // of an entry at most
   if (tiles > 0x7FFFFFFF / x.entries || tiles * x.entries > ((int64_t)1 << 38) / kv_heads)
     return fail(XT_EUNSUPPORTED, "%s: %d row tiles over a table of %d pages", what, x.entries, width);
@@ -1599,7 +1632,8 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
     if (dim == 128) return launch_decode<128, 2>(what, a, groups, stream);
     return launch_decode<256, 2>(what, a, groups, stream);
   }
-  if (dim == 64) return launch_prefill<64>(what, a, groups, stream);
-  if (dim == 128) return launch_prefill<128>(what, a, groups, stream);
-  return launch_prefill<256>(what, a, groups, stream);
+  if (m == 256) return launch_prefill<128, 8>(what, a, groups, stream);
+  if (dim == 64) return launch_prefill<64, 4>(what, a, groups, stream);
+  if (dim == 128) return launch_prefill<128, 4>(what, a, groups, stream);
+  return launch_prefill<256, 4>(what, a, groups, stream);
 }
