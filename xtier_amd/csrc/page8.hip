@@ -360,7 +360,12 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
   block_sums<T>(sum, live, s_sum, &before, &all, &cut_before, &n_live);
   // per head: the smallest size that could fit, and if it does not, one that is sure to
   const int room = max(a.slots / a.heads, 1), sure = max(max(room - n_live, room / 2), 1);
-  int size = max((all + room - 1) / room, a.min_tiles), mine, cut, per_head, cut_per_head;
+  // nor smaller than pays: n pieces of an entry of t tiles take about t / n steps and n partials to merge, whose cost grows
+  // with the rows, least at pieces of rows / 32 * sqrt(t) tiles (measured, with fixed sizes of 4 / 8 / 16 tiles:
+  // 1 request of 512 tiles, 16 rows, 21.7 / 17.6 / 17.9 us; 4 of 256 tiles, 32 rows, 38.4 / 38.3 / 28.5 us; 2 of 64
+  // tiles, 32 rows, 19.9 / 21.4 / 24.2 us)
+  const int least = max(a.min_tiles, (int)(m_rows / 32.0f * __builtin_sqrtf((float)all / max(n_live, 1))));
+  int size = max((all + room - 1) / room, least), mine, cut, per_head, cut_per_head;
   for (int tries = 0;; ++tries) {
     mine = cut = 0;
     for (int e = e0; e < e1; ++e) {
@@ -370,7 +375,7 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
     }
     block_sums<T>(mine, cut, s_sum, &before, &per_head, &cut_before, &cut_per_head);
     if (per_head <= room || tries == 1) break;
-    size = max((all + sure - 1) / sure, a.min_tiles);
+    size = max((all + sure - 1) / sure, least);
   }
   Piece x;
   x.count = 0;
@@ -623,13 +628,21 @@ __device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int he
 //
 // P and V enter the second product as FP16: P is at most 1, and V as E4M3 times 2^(its page's exponent - the largest
 // exponent seen) is exact within 15 binades below the largest. BF16 would round P eight times as coarsely.
+//
+// Workgroups on a CU at once, one wave of each to a SIMD: what the registers of O, the queries and a tile leave room for.
+constexpr int decode_per_cu(int dim) { return dim == 256 ? 1 : 2; }
+
 template <int D, int NQ>
 struct DecodeGeo {
   static constexpr int kX = D / 64;                     // 16-byte pieces of a K row per lane
   static constexpr int kDT = D / 16;                    // 16-dim tiles of O
   static constexpr int kRows = 16 * NQ;
   static constexpr int kPitch = D + 4;                  // floats of a merged row in LDS: D, max, sum, padding
-  static constexpr int kLds = 4 * kRows * kPitch * 4;
+  static constexpr int kMerge = 4 * kRows * kPitch * 4;
+  // With more than 16 rows the query operands lie in LDS, one 16-byte piece a lane for each MFMA: all waves have the same
+  // rows, and in registers they would cost a wave of each SIMD (32 rows at 128) or spills (64).
+  static constexpr int kQueries = NQ > 1 ? NQ * (D / 32) * 1024 : 0;
+  static constexpr int kLds = kMerge + kQueries;
   static constexpr int kPoison = D > 128 ? 2 : 1;       // words of D / 4 bits
 };
 
@@ -647,7 +660,7 @@ struct KvStep {
 };
 
 template <int D, int NQ>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, decode_per_cu(D)) void decode_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using G = DecodeGeo<D, NQ>;
   constexpr int M = G::kRows;
@@ -664,32 +677,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
   const int share = en.tiles / pc.count, longer = en.tiles % pc.count;    // the first `longer` pieces have a tile more
   const int t0 = pc.at * share + min(pc.at, longer), t1 = t0 + share + (pc.at < longer ? 1 : 0);
   {
-    // query operands and positions of this lane's columns
-    bf16x8_t qb[NQ][2 * G::kX];
+    // query operands and positions of this lane's columns (those past the last row repeat it with a zero query, so that
+    // they see what the others see)
+    bf16x8_t qb[NQ == 1 ? 2 * G::kX : 1];
+    uint4* const s_q = reinterpret_cast<uint4*>(s_merge + G::kMerge / 4);
     int pos[NQ];
-    int64_t q_row[NQ];
-    int q_head[NQ];
-    bool live[NQ];
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
-      const int r = en.r0 + 16 * nq + c;
-      live[nq] = r < en.r1;
-      // columns past the last row repeat it (with a zero query), so that they see what the others see
-      const int rr = live[nq] ? r : en.r1 - 1;
-      const int tok = rr / a.group;
-      q_row[nq] = en.row0 + tok;
-      q_head[nq] = head * a.group + (rr - tok * a.group);
+      const int r = en.r0 + 16 * nq + c, rr = min(r, en.r1 - 1), tok = rr / a.group;
       pos[nq] = en.start + tok;
-      const uint16_t* src = a.q + q_row[nq] * a.q_row + q_head[nq] * a.q_head + 16 * g;
+      if (NQ > 1 && nq % 4 != wave % NQ) continue;     // (each block of 16 rows by one of the waves, or by several alike)
+      const uint16_t* src = a.q + (int64_t)(en.row0 + tok) * a.q_row +
+                            (head * a.group + (rr - tok * a.group)) * a.q_head + 16 * g;
 #pragma unroll
       for (int x = 0; x < G::kX; ++x)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           uint4 w = {0, 0, 0, 0};
-          if (live[nq]) w = *reinterpret_cast<const uint4*>(src + 64 * x + 8 * y);
-          qb[nq][2 * x + y] = __builtin_bit_cast(bf16x8_t, w);
+          if (r < en.r1) w = *reinterpret_cast<const uint4*>(src + 64 * x + 8 * y);
+          if constexpr (NQ == 1) qb[2 * x + y] = __builtin_bit_cast(bf16x8_t, w);
+          else s_q[(nq * 2 * G::kX + 2 * x + y) * 64 + lane] = w;
         }
     }
+    if (NQ > 1) __syncthreads();
     const int p_lo = en.start + en.r0 / a.group, p_hi = en.start + (en.r1 - 1) / a.group;
 
     float4_t acc[NQ][G::kDT];
@@ -746,29 +756,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
     }
     // Each of the tile's registers is refilled as soon as its product has read it: the next K is on its way during
     // softmax and PV, the next V during the next scores, and the pages of the tile after that.
-    for (int t = first; t < t1; t += 4) {
+    auto step = [&](int t, auto more_tiles) {
+      constexpr bool more = decltype(more_tiles)::value;
       const int base = key_of(t);
-      const bool more = t + 4 < t1;
       // scores
       float4_t s[NQ][4];
       const float ks = exp_bits(st.ke);
 #pragma unroll
-      for (int t4 = 0; t4 < 4; ++t4) {
+      for (int t4 = 0; t4 < 4; ++t4)
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) s[nq][t4] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < G::kX; ++x) {
-          const uint4 w = st.k[x][t4];
-          const bf16x8_t k0 = e4m3x8_to_bf16(w.x, w.y, ks), k1 = e4m3x8_to_bf16(w.z, w.w, ks);
+      for (int x = 0; x < 2 * G::kX; ++x) {
+        bf16x8_t q[NQ];
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) {
-            s[nq][t4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qb[nq][2 * x], s[nq][t4], 0, 0, 0);
-            s[nq][t4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qb[nq][2 * x + 1], s[nq][t4], 0, 0, 0);
-          }
+        for (int nq = 0; nq < NQ; ++nq) {
+          if constexpr (NQ == 1) q[nq] = qb[x];
+          else q[nq] = __builtin_bit_cast(bf16x8_t, s_q[(nq * 2 * G::kX + x) * 64 + lane]);
         }
+#pragma unroll
+        for (int t4 = 0; t4 < 4; ++t4) {
+          const uint4 w = st.k[x / 2][t4];
+          const bf16x8_t k = x % 2 == 0 ? e4m3x8_to_bf16(w.x, w.y, ks) : e4m3x8_to_bf16(w.z, w.w, ks);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+            s[nq][t4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[nq], s[nq][t4], 0, 0, 0);
+        }
+        if (NQ > 1) __builtin_amdgcn_sched_barrier(0);
       }
+      // (fences to the scheduler: phases that it mixes need more registers than there are)
+      __builtin_amdgcn_sched_barrier(0);
       const bool pages_ok = st.kok && st.vok;
-      if (more) load_k(t + 4, next, st);
+      if constexpr (more) load_k(t + 4, next, st);
       // a tile that every row sees whole needs no masks
       const bool whole = base + kTile - 1 <= p_lo && base + kTile <= en.end &&
                          (a.window <= 0 || base > p_hi - a.window || base + kTile <= a.sinks) &&
@@ -786,6 +805,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
 #pragma unroll
           for (int i = 0; i < 16; ++i) mask |= sight.sees(i) ? 1u << i : 0u;
           mask = st.vok ? mask : 0u;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[nq][i >> 2][i & 3] = mask >> i & 1u ? s[nq][i >> 2][i & 3] : -__builtin_inff();
           vis[nq] = mask;
           any |= mask;
           all &= mask;
@@ -841,33 +862,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
       e_ref = e_new;
       const float vs = exp_bits(127 + max(ev - e_ref, -126));
       half8_t pb[NQ][2];
+      float f[NQ];
+      bool rescale = false;
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
-        float z[16];
         float mx = -__builtin_inff();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          z[i] = s[nq][i >> 2][i & 3] * a.scale;
-          if (!whole) z[i] = (vis[nq] >> i) & 1u ? z[i] : -__builtin_inff();
-          mx = max2_raw(mx, z[i]);
-        }
-        const float m_new = max2_raw(m_run[nq], max4_lanes16(mx));
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[nq][i >> 2][i & 3]);
+        const float m_new = fmaxf(m_run[nq], max4_lanes16(mx * a.scale));
         const float mu = m_new == -__builtin_inff() ? 0.0f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m_run[nq] - mu);
         m_run[nq] = m_new;
-        l_run[nq] *= alpha;
+        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          z[i] = __builtin_amdgcn_exp2f(z[i] - mu);
-          l_run[nq] += z[i];
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nq][i >> 2][i & 3], a.scale, -mu));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nq][i >> 2][(i & 3) + 1], a.scale, -mu));
+          sum += p0 + p1;
+          const half2_t pair = __builtin_convertvector(float2_t{p0, p1}, half2_t);
+          pb[nq][i >> 3][i & 7] = pair[0];
+          pb[nq][i >> 3][(i & 7) + 1] = pair[1];
         }
-        const float f = alpha * e_drop;
+        l_run[nq] = l_run[nq] * alpha + sum;
+        f[nq] = alpha * e_drop;
+        rescale |= f[nq] != 1.0f;
+        if (NQ > 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (__ballot(rescale)) {
 #pragma unroll
-        for (int dt = 0; dt < G::kDT; ++dt) acc[nq][dt] *= f;
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pb[nq][u][i] = (_Float16)z[8 * u + i];
+          for (int dt = 0; dt < G::kDT; ++dt) acc[nq][dt] *= f[nq];
       }
 #pragma unroll
       for (int dt = 0; dt < G::kDT; ++dt) {
@@ -878,12 +903,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
           acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pb[nq][0], acc[nq][dt], 0, 0, 0);
           acc[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pb[nq][1], acc[nq][dt], 0, 0, 0);
         }
+        if (NQ > 1 && dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
-      if (more) {
+      if constexpr (more) {
         load_v(t + 4, next, st);
-        if (t + 8 < t1) next = pages_at(t + 8);
+        next = pages_at(min(t + 8, t1 - 1));
       }
-    }
+    };
+    // (the last tile's step apart: a refill on a condition would keep two copies of the registers)
+    int t_now = first;
+    for (; t_now + 4 < t1; t_now += 4) step(t_now, std::true_type());
+    if (t_now < t1) step(t_now, std::false_type());
 
     // the waves' states, normalized and at their true scale, through LDS: rows of [O, max, sum]
     __syncthreads();
@@ -944,7 +974,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_kernel(AttnArgs 
       const int first = pc.slot - pc.at;
       int32_t* counter = a.counters + first;
       if (arrive_last(counter, pc.count, &s_last)) {
-        merge_partials<D, M, 256, 1, 16>(a, en, head, [](int w) { return w; }, first, first + pc.count - 1, pr);
+        merge_partials<D, M, 256, D == 256 ? 2 : 1, 16>(a, en, head, [](int w) { return w; }, first, first + pc.count - 1, pr);
         reset_counter(counter);
       }
     }
@@ -1438,14 +1468,19 @@ int page_shift_of(int page_size) {
                                                                                     : -1;
 }
 
-constexpr int64_t kWideRows = 256;       // rows of a request from which on 8 waves a workgroup win
 // Query rows of a workgroup, by the rows (tokens x heads of a group) that a request has on average: 16 or 32 in the
-// decode kernel, which reads its keys from memory wave by wave, else the prefill kernel's 32 for each wave: 4 waves, or 8
-// at head size 128 (at 64 a tile has too few pieces for 8 waves, at 256 a wave needs a SIMD's registers to itself).
+// decode kernel, which reads its keys from memory wave by wave, up to 64 rows of a request (2 x 32 at head size 128: 16
+// requests of 64 rows at 16K context take 79 us so, 106 as 1 x 64, whose registers leave a SIMD one wave, and 114 in the
+// prefill kernel, half empty; at head size 64, 1 x 64 takes 56 us and 2 x 32 73); above that the prefill kernel's 32 for
+// each wave: 4 waves, or 8 at head size 128 (at 64 a tile has too few pieces for 8 waves, at 256 a wave needs a SIMD's
+// registers to itself), which take 2.06 ms for 4096 tokens at 32K context where 4 take 2.25.
+constexpr int64_t kWideRows = 256;
 int tile_rows(int64_t rows, int batch, int group, int dim) {
   const int64_t all = rows * group;
-  if (all <= 32 * (int64_t)batch) return all <= 16 * (int64_t)batch ? 16 : 32;
-  return dim == 128 && all > kWideRows * (int64_t)batch ? 256 : 128;
+  if (all <= 16 * (int64_t)batch) return 16;
+  if (all <= 32 * (int64_t)batch) return 32;
+  if (all <= 64 * (int64_t)batch) return dim == 64 ? 64 : 32;
+  return dim == 128 && all > kWideRows * batch ? 256 : 128;
 }
 
 constexpr int64_t kMaxRows = 1 << 30;   // rows x heads of a group: 32-bit row numbers in the kernels
@@ -1465,8 +1500,8 @@ Launch plan_launch(int rows, int batch, int heads, int group, int dim, bool ragg
   x.m = tile_rows(rows, batch, group, dim);
   const bool prefill = x.m >= 128;
   x.entries = ragged ? (int)((int64_t)rows * group / x.m) + batch : batch * ((group + x.m - 1) / x.m);
-  // 8 waves on a CU, but 4 of the prefill kernel at head size 256
-  x.slots = (x.m == 256 || (prefill && dim == 256) ? 1 : 2) * device_cus() / 8 * 8;
+  const int per_cu = prefill ? (x.m == 256 || dim == 256 ? 1 : 2) : decode_per_cu(dim);
+  x.slots = per_cu * device_cus() / 8 * 8;
   const int64_t units = (int64_t)x.entries * heads, room = x.slots > heads ? x.slots : heads;
   x.groups = prefill ? x.slots : (int)((units + room + 7) / 8 * 8);
   x.partials = (int)(prefill ? 2 * x.slots : 2 * room);
@@ -1632,6 +1667,7 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
     if (dim == 128) return launch_decode<128, 2>(what, a, groups, stream);
     return launch_decode<256, 2>(what, a, groups, stream);
   }
+  if (m == 64) return launch_decode<64, 4>(what, a, groups, stream);
   if (m == 256) return launch_prefill<128, 8>(what, a, groups, stream);
   if (dim == 64) return launch_prefill<64, 4>(what, a, groups, stream);
   if (dim == 128) return launch_prefill<128, 4>(what, a, groups, stream);
