@@ -408,40 +408,116 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
   return x;
 }
 
-// A workgroup's work in the prefill kernel: tiles pos .. end - 1 of the launch, equal runs for all workgroups, one per
-// slot. They are bound by their arithmetic, so equal runs end together where whole units would leave slots idle.
+// The workgroup of the launch, renumbered so that each XCD (workgroups go round robin over 8) takes a contiguous run of
+// the work: neighbours in it read the same keys, out of that XCD's L2.
+__device__ inline int xcd_order(int id, int groups) { return (id & 7) * (groups >> 3) + (id >> 3); }
+
+// A workgroup's work in the prefill kernel, which has one workgroup to a slot: segments, each the tiles t0 .. t1 - 1 of
+// one (head, entry). Its `sharers` workgroups leave partials in slots base + step * i (the first one's moved by `bump`).
+//
+// Either the work is dealt out in pieces, whole entries or (with fewer of them than slots) even cuts of them, or, where
+// that would leave slots idle in the last round, every workgroup takes an equal run of tiles, across entries. An entry
+// costs about kStart tiles to begin and end, and kShare more where its partials go through memory (measured: 8 and 24 us
+// of 2.1 us a tile at 256 rows x 128, 6 and 9 us of 1 us at 128 x 64), by which the cheaper way is chosen. Runs alone: 2
+// prompts of 1024 tokens, 32 / 4 heads x 128, 118 us, 5 prompts through a window of 1000, 106 us; with the choice
+// 55 and 86 us (with the cheaper masks that came with it).
 //
 // (What is the same in every lane but comes out of LDS goes through readfirstlane, in both kernels: the loads of an entry
 // are then scalar loads, and the loops over tiles and their branches scalar ones.)
-struct Share {
-  int per, per_head;              // tiles of a workgroup, of one head
-  int64_t total, pos, end;        // tiles of the launch; this workgroup's run
-  int head;
-  int entry, entry_pos;           // the entry that holds pos, and the number of its first tile within its head
+constexpr int kStart = 4, kShare = 10;
+struct Run {
+  bool pieces;
+  int per_head;                        // pieces of a head, or its tiles
+  int size, cut_per_head;              // pieces: of at most `size` tiles, those of cut entries
+  int turn;                            // pieces this workgroup has had
+  int per, entry_pos;                  // runs: tiles of one, and the first tile of the entry within its head
+  int64_t pos, end;
+};
+struct Segment {
+  int head, entry, t0, t1;
+  int sharers, at;                     // at: this workgroup among them
+  int base, step, bump, counter;
+  __device__ int slot(int i) const { return base + step * i + (i == 0 ? bump : 0); }
 };
 
 template <int T>
-__device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int group_id) {
-  __shared__ int s_sum[2 * (T / 64)];
-  __shared__ int s_find[2];
-  Share sh;
+__device__ inline Run plan_run(const AttnArgs& a, int m_rows, int groups, int id, int* s_sum, int* s_find, int* s_mine,
+                                Segment* sg) {
+  Run x;
   const int tid = (int)threadIdx.x;
   const int chunk = (a.entries + T - 1) / T;
   const int e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
-  int sum = 0, before, all, unused, none;
-  for (int e = e0; e < e1; ++e) sum += entry_at(a, e, m_rows).tiles;
-  block_sums<T>(sum, 0, s_sum, &before, &all, &unused, &none);
+  int sum = 0, live = 0, most = 0, before, all, cut_before, n_live;
+  for (int e = e0; e < e1; ++e) {
+    const int t = entry_at(a, e, m_rows).tiles;
+    sum += t;
+    live += t > 0;
+    most = max(most, t);
+  }
+  if (tid == 0) s_find[0] = 0;
+  block_sums<T>(sum, live, s_sum, &before, &all, &cut_before, &n_live);
+  atomicMax(&s_find[0], most);
+  __syncthreads();
+  most = __builtin_amdgcn_readfirstlane(s_find[0]);
   all = __builtin_amdgcn_readfirstlane(all);
-  sh.per_head = all;
-  sh.total = (int64_t)all * a.heads;
-  sh.per = (int)((sh.total + groups - 1) / groups);
-  if (sh.per < a.min_tiles) sh.per = a.min_tiles;
-  sh.pos = (int64_t)sh.per * group_id;
-  sh.end = min(sh.pos + sh.per, sh.total);
-  sh.head = sh.entry = sh.entry_pos = 0;
-  if (sh.pos >= sh.end) return sh;
-  sh.head = (int)(sh.pos / all);
-  const int want = (int)(sh.pos - (int64_t)sh.head * all);   // within the head
+  n_live = __builtin_amdgcn_readfirstlane(n_live);
+  const int units = n_live * a.heads;
+  const int64_t total = (int64_t)all * a.heads;
+  // steps until the last workgroup is done: runs, whole entries in rounds (the last of them with the longest entry), or
+  // entries cut so that all pieces are on the CUs at once
+  const int run = (int)((total + groups - 1) / groups);
+  const int per_slot = (units + groups - 1) / groups;
+  const float by_runs = (float)run + (1.0f + (float)units / groups) * kStart + 1.5f * kShare;
+  const float mean = (float)total / max(units, 1);
+  const float whole = per_slot * (mean + kStart) + 0.5f * ((float)most - mean);
+  const int spare = units < groups ? (groups - units) / a.heads : 0;
+  int size = most;
+  float by_pieces = whole;
+  if (spare > 0) {
+    const int cut = max((all + spare - 1) / spare, a.min_tiles);
+    if (cut < most && cut + kStart + kShare < whole) {
+      size = cut;
+      by_pieces = (float)(cut + kStart + kShare);
+    }
+  }
+  x.pieces = by_pieces <= by_runs;
+  x.turn = 0;
+  x.per = max(run, a.min_tiles);
+  x.pos = x.end = 0;
+  x.per_head = all;
+  sg->head = sg->entry = sg->t0 = sg->t1 = 0;
+  if (x.pieces) {
+    // s_mine: of each thread's entries, the pieces before them, theirs, and the cut ones before them (in LDS: in
+    // registers they would stay through the whole kernel)
+    int mine, cut;
+    const int room = max(groups / a.heads, 1), tight = max((all + room - 1) / room, a.min_tiles);
+    const bool try_tight = size < most && tight < size;      // the smallest size that could fit, else the sure one
+    for (int tries = try_tight ? 0 : 1;; ++tries) {
+      x.size = max(tries == 0 ? tight : size, 1);
+      mine = cut = 0;
+      for (int e = e0; e < e1; ++e) {
+        const int n = (entry_at(a, e, m_rows).tiles + x.size - 1) / x.size;
+        mine += n;
+        cut += n > 1 ? n : 0;
+      }
+      block_sums<T>(mine, cut, s_sum, &before, &x.per_head, &cut_before, &x.cut_per_head);
+      if (tries == 1 || __builtin_amdgcn_readfirstlane(x.per_head) <= room) break;
+    }
+    x.size = __builtin_amdgcn_readfirstlane(x.size);
+    s_mine[tid] = before;
+    s_mine[T + tid] = mine;
+    s_mine[2 * T + tid] = cut_before;
+    x.per_head = __builtin_amdgcn_readfirstlane(x.per_head);
+    x.cut_per_head = __builtin_amdgcn_readfirstlane(x.cut_per_head);
+    return x;
+  }
+  const int w = xcd_order(id, groups);
+  x.pos = (int64_t)x.per * w;
+  x.end = min(x.pos + x.per, total);
+  if (x.pos >= x.end) return x;
+  sg->head = (int)(x.pos / all);
+  const int want = (int)(x.pos - (int64_t)sg->head * all);   // within the head
+  __syncthreads();
   if (want >= before && want < before + sum) {
     int at = before;
     for (int e = e0; e < e1; ++e) {
@@ -455,27 +531,78 @@ __device__ inline Share share_of(const AttnArgs& a, int m_rows, int groups, int 
     }
   }
   __syncthreads();
-  sh.entry = __builtin_amdgcn_readfirstlane(s_find[0]);
-  sh.entry_pos = __builtin_amdgcn_readfirstlane(s_find[1]);
-  return sh;
+  sg->entry = __builtin_amdgcn_readfirstlane(s_find[0]);
+  x.entry_pos = __builtin_amdgcn_readfirstlane(s_find[1]);
+  return x;
 }
 
-// The workgroup of the launch, renumbered so that each XCD (workgroups go round robin over 8) takes a contiguous run of
-// the work: neighbours in it read the same keys, out of that XCD's L2.
-__device__ inline int xcd_order(int id, int groups) { return (id & 7) * (groups >> 3) + (id >> 3); }
-
-// On to the run's next entry that has rows, after the tiles of `sh.entry` up to t1 (unit0: its first tile).
-__device__ inline void next_entry(const AttnArgs& a, Share& sh, int64_t unit0, int t1, int tiles, int m_rows) {
-  sh.pos = unit0 + t1;
-  if (sh.pos >= sh.end) return;
-  sh.entry_pos += tiles;
-  do {
-    if (++sh.entry == a.entries) {
-      sh.entry = 0;
-      sh.entry_pos = 0;
-      ++sh.head;
+// The workgroup's next segment and its entry; false when there is none.
+template <int T>
+__device__ inline bool next_segment(const AttnArgs& a, int m_rows, int groups, int id, int* s_find, const int* s_mine, Run& x,
+                                    Segment* sg, Entry* en) {
+  if (x.pieces) {
+    // each XCD (workgroups go round robin over 8) takes an eighth of the pieces, neighbours in the same keys together
+    const int count = x.per_head * a.heads, of_xcd = (count + 7) / 8;
+    const int turn = (id >> 3) + x.turn * (groups >> 3), w = (id & 7) * of_xcd + turn;
+    ++x.turn;
+    if (turn >= of_xcd || w >= count) return false;
+    sg->head = w / x.per_head;
+    const int tid = (int)threadIdx.x;
+    int want = w - sg->head * x.per_head - s_mine[tid], rank = s_mine[2 * T + tid];
+    __syncthreads();
+    if (want >= 0 && want < s_mine[T + tid]) {
+      const int chunk = (a.entries + T - 1) / T, e0 = chunk * tid;
+      for (int e = e0; e < min(e0 + chunk, a.entries); ++e) {
+        const int n = (entry_at(a, e, m_rows).tiles + x.size - 1) / x.size;
+        if (want < n) {
+          s_find[0] = e;
+          s_find[1] = want;
+          s_find[2] = n;
+          s_find[3] = rank;
+          break;
+        }
+        want -= n;
+        rank += n > 1 ? n : 0;
+      }
     }
-  } while (entry_at(a, sh.entry, m_rows).tiles == 0);
+    __syncthreads();
+    sg->entry = __builtin_amdgcn_readfirstlane(s_find[0]);
+    sg->at = __builtin_amdgcn_readfirstlane(s_find[1]);
+    sg->sharers = __builtin_amdgcn_readfirstlane(s_find[2]);
+    *en = entry_at(a, sg->entry, m_rows);
+    const int share = en->tiles / sg->sharers, longer = en->tiles % sg->sharers;   // the first `longer` have one more
+    sg->t0 = sg->at * share + min(sg->at, longer);
+    sg->t1 = sg->t0 + share + (sg->at < longer ? 1 : 0);
+    sg->base = sg->counter = sg->head * x.cut_per_head + __builtin_amdgcn_readfirstlane(s_find[3]);
+    sg->step = 1;
+    sg->bump = 0;
+    return true;
+  }
+  if (x.pos >= x.end) return false;
+  if (sg->t1 > 0) {                    // on to the next entry that has rows
+    x.entry_pos += en->tiles;
+    do {
+      if (++sg->entry == a.entries) {
+        sg->entry = 0;
+        x.entry_pos = 0;
+        ++sg->head;
+      }
+    } while (entry_at(a, sg->entry, m_rows).tiles == 0);
+  }
+  *en = entry_at(a, sg->entry, m_rows);
+  const int64_t first = (int64_t)sg->head * x.per_head + x.entry_pos;       // the entry's first tile
+  sg->t0 = (int)(x.pos - first);
+  sg->t1 = (int)min((int64_t)en->tiles, x.end - first);
+  x.pos = first + sg->t1;
+  // a workgroup has two slots: for an entry that began before its run, and for one that ends after it
+  const int w0 = (int)(first / x.per);
+  sg->sharers = (int)((first + en->tiles - 1) / x.per) - w0 + 1;
+  sg->at = xcd_order(id, groups) - w0;
+  sg->base = 2 * w0;
+  sg->step = 2;
+  sg->bump = (int64_t)x.per * w0 < first ? 1 : 0;
+  sg->counter = w0;
+  return true;
 }
 
 __device__ inline void store_out(const AttnArgs& a, int64_t row, int head, int d, float4_t v) {
@@ -494,8 +621,17 @@ __device__ inline void store_out(const AttnArgs& a, int64_t row, int head, int d
 // The keys that a row at position p sees, as bounds on j - base: j < hi and (j >= lo or j < sink).
 struct Sight {
   int hi, lo, sink;
-  __device__ bool sees(int i) const { return (i < hi) & ((i >= lo) | (i < sink)); }
+  // for j - base = from .. from + n - 1, n <= 16, as bits
+  __device__ uint32_t bits(int from, int n) const {
+    auto below = [&](int x) { return (1u << min(max(x - from, 0), n)) - 1u; };
+    return below(hi) & (~below(lo) | below(sink));
+  }
 };
+// x where bit i of mask is set, -inf elsewhere.
+__device__ inline float unless_hidden(float x, uint32_t mask, int i) {
+  const uint32_t keep = (uint32_t)((int32_t)(mask << (31 - i)) >> 31);
+  return __uint_as_float((__float_as_uint(x) & keep) | (0xFF800000u & ~keep));
+}
 __device__ inline Sight sight_of(const AttnArgs& a, int p_hi, int p_lo, int end, int base) {
   Sight x;
   x.hi = min(p_hi + 1, end) - base;
@@ -551,11 +687,11 @@ __device__ inline float lse_of(float m, float l) {
 }
 
 // The last workgroup of a (head, entry) merges its partials, slots of [rows][D O values, max, sum, padding]: normalized
-// outputs, their maximum (of scaled scores in base 2) and their sum relative to it. slot_of(w): workgroup w's slot.
+// outputs, their maximum (of scaled scores in base 2) and their sum relative to it. slot_of(i): the i-th one's slot.
 // Reads miss every cache, so a thread has those of UB pieces of CB workgroups in flight at once.
 template <int D, int M, int T, int UB, int CB, typename SlotOf>
-__device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int head, SlotOf slot_of,
-                                      int w_first, int w_last, __amdgpu_buffer_rsrc_t pr) {
+__device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int head, SlotOf slot_of, int sharers,
+                                      __amdgpu_buffer_rsrc_t pr) {
   constexpr int kPieces = D / 4, kPitch = D + 4, kSlot = M * kPitch;
   const int units = (en.r1 - en.r0) * kPieces;
   for (int i0 = (int)threadIdx.x; i0 < units; i0 += T * UB) {
@@ -567,7 +703,7 @@ __device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int he
       l[k] = 0.0f;
       o[k] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    for (int w0 = w_first; w0 <= w_last; w0 += CB) {
+    for (int w0 = 0; w0 < sharers; w0 += CB) {
       float4_t ml[UB][CB], x[UB][CB];
 #pragma unroll
       for (int k = 0; k < UB; ++k)
@@ -576,7 +712,7 @@ __device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int he
           const int w = w0 + c;
           const int i = i0 + k * T;
           // (past the last workgroup or piece: an offset past the buffer, which reads zeros)
-          const bool real = w <= w_last && i < units;
+          const bool real = w < sharers && i < units;
           const int at = real ? (slot_of(w) * kSlot + i / kPieces * kPitch) * 4 : -16;
           ml[k][c] = load_partial(pr, real ? at + 4 * D : -16);
           x[k][c] = load_partial(pr, real ? at + i % kPieces * 16 : -16);
@@ -801,12 +937,9 @@ __global__ __launch_bounds__(256, decode_per_cu(D)) void decode_kernel(AttnArgs 
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
           const Sight sight = sight_of(a, pos[nq], pos[nq], en.end, j0);
-          uint32_t mask = 0;
+          const uint32_t mask = st.vok ? sight.bits(0, 16) : 0u;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mask |= sight.sees(i) ? 1u << i : 0u;
-          mask = st.vok ? mask : 0u;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[nq][i >> 2][i & 3] = mask >> i & 1u ? s[nq][i >> 2][i & 3] : -__builtin_inff();
+          for (int i = 0; i < 16; ++i) s[nq][i >> 2][i & 3] = unless_hidden(s[nq][i >> 2][i & 3], mask, i);
           vis[nq] = mask;
           any |= mask;
           all &= mask;
@@ -974,7 +1107,7 @@ __global__ __launch_bounds__(256, decode_per_cu(D)) void decode_kernel(AttnArgs 
       const int first = pc.slot - pc.at;
       int32_t* counter = a.counters + first;
       if (arrive_last(counter, pc.count, &s_last)) {
-        merge_partials<D, M, 256, D == 256 ? 2 : 1, 16>(a, en, head, [](int w) { return w; }, first, first + pc.count - 1, pr);
+        merge_partials<D, M, 256, D == 256 ? 2 : 1, 16>(a, en, head, [&](int i) { return first + i; }, pc.count, pr);
         reset_counter(counter);
       }
     }
@@ -1038,19 +1171,19 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
   __shared__ __attribute__((aligned(16))) uint16_t s_where[2][D][4];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hf = lane >> 5;
+  __shared__ int s_sum[2 * (T / 64)];
+  __shared__ int s_find[4];
+  __shared__ int s_mine[3 * T];
   const int groups = (int)gridDim.x;
-  const int wg = xcd_order((int)blockIdx.x, groups);
-  Share sh = share_of<T>(a, M, groups, wg);
+  Segment sg;
+  Entry en;
+  Run run = plan_run<T>(a, M, groups, (int)blockIdx.x, s_sum, s_find, s_mine, &sg);
   const int page_mask = (1 << a.page_shift) - 1;
   uint8_t* const s_k = s_stage;                       // [2][64 keys] rows of D BF16
   uint8_t* const s_v = s_stage + 2 * G::kStageK;      // [2][D] rows of 64 keys, FP16
 
-  while (sh.pos < sh.end) {
-    const Entry en = entry_at(a, sh.entry, M);
-    const int64_t unit0 = (int64_t)sh.head * sh.per_head + sh.entry_pos;
-    const int t0 = (int)(sh.pos - unit0);
-    const int t1 = (int)min((int64_t)en.tiles, sh.end - unit0);
-    const int head = sh.head;
+  while (next_segment<T>(a, M, groups, (int)blockIdx.x, s_find, s_mine, run, &sg, &en)) {
+    const int t0 = sg.t0, t1 = sg.t1, head = sg.head;
 
     const int r = en.r0 + 32 * wave + c;
     const bool live = r < en.r1;
@@ -1162,13 +1295,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
         // values of keys that no row sees may be anything, NaN included: zero them
         const int j0 = key_of(min(t, t1 - 1)) + 16 * (tid & 3);
         const Sight widest = sight_of(a, p_hi, p_lo, en.end, j0), least = sight_of(a, p_lo, p_hi, en.end, j0);
-        uint32_t any = 0, all = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          any |= widest.sees(i) ? 1u << i : 0u;
-          all |= least.sees(i) ? 1u << i : 0u;
-        }
-        if (!vok) any = 0;
+        const uint32_t any = vok ? widest.bits(0, 16) : 0u, all = least.bits(0, 16);
         if (any == 0) ev = -1;
         const uint32_t some = any & ~all;
         uint32_t nan = 0;
@@ -1293,17 +1420,14 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
       // s[kb][4 a + i] is key base + 32 kb + 16 (a / 2) + 8 hf + 4 (a % 2) + i
       uint32_t vis = 0xFFFFFFFFu;
       if (!whole_tile(t) || tile_ok != 15u) {
-        vis = 0;
+        vis = 0;                              // bit 16 kb + i
         const Sight sight = sight_of(a, pos, pos, en.end, key_of(t) + 8 * hf);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) vis |= (tile_ok >> u & 1u ? sight.bits(16 * u, 8) : 0u) << (8 * u);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int in_tile = 32 * kb + 16 * (i >> 3) + (i & 7);
-            const bool see = sight.sees(in_tile) & ((tile_ok >> (in_tile >> 4) & 1u) != 0);
-            vis |= see ? 1u << (16 * kb + i) : 0u;
-            s[kb][i] = see ? s[kb][i] : -__builtin_inff();
-          }
+          for (int i = 0; i < 16; ++i) s[kb][i] = unless_hidden(s[kb][i], vis, 16 * kb + i);
       }
       // scores of the next tile beside this one's softmax: a quarter of the chunks for the maximum, the others for the
       // exponentials
@@ -1420,10 +1544,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
 
     // every wave has its rows whole: outputs or partials straight from registers (acc[dt][4 a + i] is dimension
     // 32 dt + 8 a + 4 hf + i)
-    const int w_first = (int)(unit0 / sh.per), w_last = (int)((unit0 + en.tiles - 1) / sh.per);
-    const bool alone = w_first == w_last;
-    // a workgroup's partials: of an entry that began before its run, and of one that ends after it
-    auto slot_of = [&](int w) { return 2 * w + ((int64_t)sh.per * w < unit0 ? 1 : 0); };
+    const bool alone = sg.sharers == 1;
     const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
         a.part, (short)0, (int)min((int64_t)a.partials * kSlot * 4, (int64_t)0x7FFFFFFF), 0x00020000);
     float l = l_run;
@@ -1432,7 +1553,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
       l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     }
     const float f = l != 0.0f ? exp_bits(e_ref) / l : 0.0f;
-    const int my_slot = slot_of(wg);
+    const int my_slot = sg.slot(sg.at);
     if (live) {
 #pragma unroll
       for (int dt = 0; dt < G::kDT; ++dt)
@@ -1452,13 +1573,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
       }
     }
     if (!alone) {
-      int32_t* counter = a.counters + w_first;
-      if (arrive_last(counter, w_last - w_first + 1, &s_last)) {
-        merge_partials<D, M, T, 4, 4>(a, en, head, slot_of, w_first, w_last, pr);
+      int32_t* counter = a.counters + sg.counter;
+      if (arrive_last(counter, sg.sharers, &s_last)) {
+        merge_partials<D, M, T, 4, 4>(a, en, head, [&](int i) { return sg.slot(i); }, sg.sharers, pr);
         reset_counter(counter);
       }
     }
-    next_entry(a, sh, unit0, t1, en.tiles, M);
   }
 #endif
 }
@@ -1474,13 +1594,12 @@ int page_shift_of(int page_size) {
 // prefill kernel, half empty; at head size 64, 1 x 64 takes 56 us and 2 x 32 73); above that the prefill kernel's 32 for
 // each wave: 4 waves, or 8 at head size 128 (at 64 a tile has too few pieces for 8 waves, at 256 a wave needs a SIMD's
 // registers to itself), which take 2.06 ms for 4096 tokens at 32K context where 4 take 2.25.
-constexpr int64_t kWideRows = 256;
 int tile_rows(int64_t rows, int batch, int group, int dim) {
   const int64_t all = rows * group;
   if (all <= 16 * (int64_t)batch) return 16;
   if (all <= 32 * (int64_t)batch) return 32;
   if (all <= 64 * (int64_t)batch) return dim == 64 ? 64 : 32;
-  return dim == 128 && all > kWideRows * batch ? 256 : 128;
+  return dim == 128 ? 256 : 128;
 }
 
 constexpr int64_t kMaxRows = 1 << 30;   // rows x heads of a group: 32-bit row numbers in the kernels
@@ -1670,6 +1789,5 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
   if (m == 64) return launch_decode<64, 4>(what, a, groups, stream);
   if (m == 256) return launch_prefill<128, 8>(what, a, groups, stream);
   if (dim == 64) return launch_prefill<64, 4>(what, a, groups, stream);
-  if (dim == 128) return launch_prefill<128, 4>(what, a, groups, stream);
   return launch_prefill<256, 4>(what, a, groups, stream);
 }
