@@ -343,8 +343,65 @@ struct Piece {
   int slot;              // of the piece's partial, if count > 1; the slots of an entry's pieces are neighbours
 };
 
+// The smallest piece that pays: n pieces of an entry of t tiles take about t / n steps and n partials to merge, whose cost
+// grows with the rows, least at pieces of rows / 32 * sqrt(t) tiles (measured, with fixed sizes of 4 / 8 / 16 tiles: 1
+// request of 512 tiles, 16 rows, 21.7 / 17.6 / 17.9 us; 4 of 256 tiles, 32 rows, 38.4 / 38.3 / 28.5 us; 2 of 64 tiles, 32
+// rows, 19.9 / 21.4 / 24.2 us). 16 partials are read in one go, so a few more than 16 pieces become 16.
+__device__ inline int least_piece(const AttnArgs& a, int m_rows, int all, int n_live) {
+  const int t = all / max(n_live, 1);
+  const int size = max(a.min_tiles, (int)(m_rows / 32.0f * __builtin_sqrtf((float)t))), n = (t + size - 1) / size;
+  return n > 16 && n < 24 ? (t + 15) / 16 : size;
+}
+
+// Which piece a workgroup of the grid takes, of `count`: each XCD (workgroups go round robin over 8) takes an eighth of
+// the pieces, neighbours in the same keys together; the grid has room for more pieces than there are, so the eighths
+// are of what there is. -1: none.
+__device__ inline int piece_of_xcd(int id, int count) {
+  const int of_xcd = (count + 7) / 8, w = (id & 7) * of_xcd + (id >> 3);
+  return (id >> 3) < of_xcd && w < count ? w : -1;
+}
+
 template <int T>
 __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
+  Piece x;
+  x.count = 0;
+  const int room = max(a.slots / a.heads, 1);       // pieces of a head
+  if (a.entries <= 64) {
+    // an entry to a lane, every wave by itself: no barriers (1 request of 4099 keys, 18.5 us with them, 17.3 without)
+    const int lane = (int)threadIdx.x & 63;
+    const int tiles = lane < a.entries ? entry_at(a, lane, m_rows).tiles : 0;
+    int all = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    const int n_live = __popcll(__ballot(tiles > 0)), sure = max(max(room - n_live, room / 2), 1);
+    const int least = least_piece(a, m_rows, all, n_live);
+    int size = max((all + room - 1) / room, least), n, upto, cut;
+    for (int tries = 0;; ++tries) {
+      n = (tiles + size - 1) / size;
+      upto = n;
+      cut = n > 1 ? n : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(upto, d), v = __shfl_up(cut, d);
+        if (lane >= d) {
+          upto += u;
+          cut += v;
+        }
+      }
+      if (__builtin_amdgcn_readlane(upto, 63) <= room || tries == 1) break;
+      size = max((all + sure - 1) / sure, least);
+    }
+    const int per_head = __builtin_amdgcn_readlane(upto, 63), cut_per_head = __builtin_amdgcn_readlane(cut, 63);
+    const int w = piece_of_xcd(id, per_head * a.heads);
+    if (w < 0) return x;
+    x.head = w / per_head;
+    const int want = w - x.head * per_head;
+    x.entry = __builtin_ctzll(__ballot(want < upto));          // the first entry whose running count passes it
+    x.count = __builtin_amdgcn_readlane(n, x.entry);
+    x.at = want - (__builtin_amdgcn_readlane(upto, x.entry) - x.count);
+    x.slot = x.head * cut_per_head + __builtin_amdgcn_readlane(cut, x.entry) - x.count + x.at;
+    return x;
+  }
   __shared__ int s_sum[2 * (T / 64)];
   __shared__ int s_find[4];
   const int tid = (int)threadIdx.x;
@@ -359,12 +416,7 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
   auto tiles_of = [&](int e) { return chunk == 1 ? tiles : entry_at(a, e, m_rows).tiles; };
   block_sums<T>(sum, live, s_sum, &before, &all, &cut_before, &n_live);
   // per head: the smallest size that could fit, and if it does not, one that is sure to
-  const int room = max(a.slots / a.heads, 1), sure = max(max(room - n_live, room / 2), 1);
-  // nor smaller than pays: n pieces of an entry of t tiles take about t / n steps and n partials to merge, whose cost grows
-  // with the rows, least at pieces of rows / 32 * sqrt(t) tiles (measured, with fixed sizes of 4 / 8 / 16 tiles:
-  // 1 request of 512 tiles, 16 rows, 21.7 / 17.6 / 17.9 us; 4 of 256 tiles, 32 rows, 38.4 / 38.3 / 28.5 us; 2 of 64
-  // tiles, 32 rows, 19.9 / 21.4 / 24.2 us)
-  const int least = max(a.min_tiles, (int)(m_rows / 32.0f * __builtin_sqrtf((float)all / max(n_live, 1))));
+  const int sure = max(max(room - n_live, room / 2), 1), least = least_piece(a, m_rows, all, n_live);
   int size = max((all + room - 1) / room, least), mine, cut, per_head, cut_per_head;
   for (int tries = 0;; ++tries) {
     mine = cut = 0;
@@ -377,12 +429,8 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
     if (per_head <= room || tries == 1) break;
     size = max((all + sure - 1) / sure, least);
   }
-  Piece x;
-  x.count = 0;
-  // each XCD (workgroups go round robin over 8) takes an eighth of the pieces, neighbours in the same keys together; the
-  // grid has room for more pieces than there are, so the eighths are of what there is
-  const int of_xcd = (per_head * a.heads + 7) / 8, w = (id & 7) * of_xcd + (id >> 3);
-  if ((id >> 3) >= of_xcd || w >= per_head * a.heads) return x;
+  const int w = piece_of_xcd(id, per_head * a.heads);
+  if (w < 0) return x;
   x.head = w / per_head;
   int want = w - x.head * per_head - before;        // the piece, counted from this thread's first
   if (want >= 0 && want < mine) {
@@ -541,11 +589,9 @@ template <int T>
 __device__ inline bool next_segment(const AttnArgs& a, int m_rows, int groups, int id, int* s_find, const int* s_mine, Run& x,
                                     Segment* sg, Entry* en) {
   if (x.pieces) {
-    // each XCD (workgroups go round robin over 8) takes an eighth of the pieces, neighbours in the same keys together
-    const int count = x.per_head * a.heads, of_xcd = (count + 7) / 8;
-    const int turn = (id >> 3) + x.turn * (groups >> 3), w = (id & 7) * of_xcd + turn;
+    const int w = piece_of_xcd(id + x.turn * groups, x.per_head * a.heads);
     ++x.turn;
-    if (turn >= of_xcd || w >= count) return false;
+    if (w < 0) return false;
     sg->head = w / x.per_head;
     const int tid = (int)threadIdx.x;
     int want = w - sg->head * x.per_head - s_mine[tid], rank = s_mine[2 * T + tid];

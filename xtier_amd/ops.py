@@ -1246,7 +1246,7 @@ def page8_attention(q, raw, table, seq_lens, scale, cu_q=None, window=0, sinks=0
         with torch.cuda.device(away):
             return page8_attention(q, raw, table, seq_lens, scale, cu_q, window, sinks, out, lse, ws)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os, out_dtype = out.stride(), _lib.XT_DTYPE_BF16
     else:
         os, out_dtype = out.stride(), _DTYPES.get(out.dtype)
