@@ -418,8 +418,8 @@ int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
  * first. Only full pages are ever shared, so a row may append to its last page. Rows, table entries and ids outside
  * their range are left alone. page_size: a power of 2. */
 
-/* Device workspace of xt_pages_extend (forks 0), xt_pages_fork and xt_pages_compact (forks 0). */
-size_t xt_pages_workspace_bytes(int64_t pages, int forks);
+/* Device workspace of xt_pages_extend and xt_pages_compact. */
+size_t xt_pages_workspace_bytes(int64_t pages);
 
 /* Each row b grows by add[b] >= 0 tokens: it gets the pages that ceil((lens[b] + add[b]) / page_size) columns need, and
  * lens[b] += add[b]. Rows are served in order: a row whose pages, with those that the rows before it asked for, are more
@@ -433,7 +433,9 @@ int xt_pages_extend(int32_t* refs, int64_t pages, int32_t* table, int64_t table_
  * page of its own, dst, to which the caller copies src in every layer (xt_pages_copy): moves[i] = src,
  * moves[moves_stride + i] = dst, both -1 where nothing is to be copied. Without a free page left (they are given in
  * order) the child gets the full pages' tokens only. Lengths are those before the call. A fork is skipped if a row id is
- * out of range, if the child holds tokens, or if an earlier fork of the call names the same child. forks <= 1024. */
+ * out of range, if the child holds tokens, or if an earlier fork of the call names the same child. forks <= 1024.
+ * workspace: 12 bytes a fork where forks * width > XT_PAGES_FORK_CELLS, else none (NULL). */
+#define XT_PAGES_FORK_CELLS 16384
 int xt_pages_fork(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width, int32_t* lens, int rows,
                   int page_size, const int32_t* parents, const int32_t* children, int forks, int32_t* moves,
                   int64_t moves_stride, void* workspace, size_t workspace_bytes, xt_stream_t stream);

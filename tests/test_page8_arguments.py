@@ -66,8 +66,7 @@ def test_attention(lib):
 
 def test_page_operators(lib):
     ok, bad, small, far = _lib.XT_OK, _lib.XT_EINVAL, _lib.XT_EWORKSPACE, _lib.XT_EUNSUPPORTED
-    need = lib.xt_pages_workspace_bytes(100, 7)
-    assert need >= 400 and lib.xt_pages_workspace_bytes(-1, 0) == 0
+    assert lib.xt_pages_workspace_bytes(100) == 400 and lib.xt_pages_workspace_bytes(-1) == 0
     extend = lambda refs=P, pages=100, table=P, ts=9, w=9, lens=P, add=P, rows=3, page=16, g=P, ws=P, n=400: \
         lib.xt_pages_extend(refs, pages, table, ts, w, lens, add, rows, page, g, ws, n, None)
     assert extend(rows=0) == ok
@@ -75,9 +74,10 @@ def test_page_operators(lib):
                dict(w=0), dict(ts=8), dict(rows=-1), dict(page=0), dict(page=12), dict(page=-16)):
         assert extend(**kw) == bad, kw
     assert extend(ws=None) == small and extend(n=399) == small
-    fork = lambda forks=7, p=P, c=P, moves=P, ms=7, n=need, page=16: \
-        lib.xt_pages_fork(P, 100, P, 9, 9, P, 3, page, p, c, forks, moves, ms, P, n, None)
-    assert fork(forks=0) == ok and fork(forks=1025, ms=1025) == far and fork(n=need - 1) == small
+    fork = lambda forks=7, p=P, c=P, moves=P, ms=7, n=0, page=16, w=9: \
+        lib.xt_pages_fork(P, 100, P, w, w, P, 3, page, p, c, forks, moves, ms, P, n, None)
+    assert fork(forks=0) == ok and fork(forks=1025, ms=1025) == far
+    assert fork(w=2341, n=7 * 12 - 1) == small                        # 7 * 2341 columns: past the one-launch size
     for kw in (dict(p=None), dict(c=None), dict(moves=None), dict(ms=6), dict(forks=-1), dict(page=3)):
         assert fork(**kw) == bad, kw
     assert lib.xt_pages_free(P, 100, P, 9, 9, P, 3, None, 0, None) == ok

@@ -53,7 +53,7 @@ class PageBuffer(ctypes.Structure):
 _CP, _KP, _FP = ctypes.POINTER(MlaCache), ctypes.POINTER(MlaKeys), ctypes.POINTER(MlaFp8Cache)
 _SP = ctypes.POINTER(KvStore)
 _BP = ctypes.POINTER(PageBuffer)
-PAGES_COPY_MAX = 64
+PAGES_COPY_MAX, PAGES_FORK_CELLS = 64, 16384
 
 SIGNATURES = {
     'xt_version': (_I, []),
@@ -91,7 +91,7 @@ SIGNATURES = {
     'xt_page8_attention_workspace_bytes': (_Z, [_I, _I, _I, _I, _I]),
     'xt_page8_attention': (_I, [_P, _L, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _L, _L, _L, _L, _P, _L, _I, _P, _P, _I,
                                 _I, _I, _I, _F, _P, _L, _L, _I, _P, _P, _Z, _P]),
-    'xt_pages_workspace_bytes': (_Z, [_L, _I]),
+    'xt_pages_workspace_bytes': (_Z, [_L]),
     'xt_pages_extend': (_I, [_P, _L, _P, _L, _I, _P, _P, _I, _I, _P, _P, _Z, _P]),
     'xt_pages_fork': (_I, [_P, _L, _P, _L, _I, _P, _I, _I, _P, _P, _I, _P, _L, _P, _Z, _P]),
     'xt_pages_free': (_I, [_P, _L, _P, _L, _I, _P, _I, _P, _I, _P]),

@@ -69,13 +69,19 @@ __device__ inline uint32_t e4m3_pair(float a, float b) {
 #endif
 }
 
-// One workgroup per (touched page, head). The page's new rows are read twice, once for their largest magnitude and once
-// to quantize them (the second time from L2).
+// One workgroup per (touched page, head, K or V). A thread keeps its first kKeep 16-byte pieces of the new rows in
+// registers between the largest magnitude and the conversion; of larger pages the rest is read again, from L2. The rows'
+// addresses do not depend on the page, so their loads go out before the table's answer is in. V is transposed through
+// LDS. Bound by the chain of loads and the launch: measured 4.5 us for one row each of 32 requests (4 heads
+// x 128), 9.3 for a chunk of 4096, 8.8 for 24 requests of up to 300 (2 x 256, pages of 16).
+constexpr int kKeep = 4;
+
 template <int T>
 __global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t s_vt[];   // [dim][page + 4] bytes of the new V rows
-  __shared__ uint32_t s_mag[2];
-  const int head = (int)blockIdx.y;
+  __shared__ uint32_t s_mag;
+  const int head = (int)blockIdx.y, tid = (int)threadIdx.x;
+  const bool is_v = blockIdx.z == 1;
   const int64_t unit = blockIdx.x;
   const int page = 1 << a.page_shift;
   int b;
@@ -104,17 +110,26 @@ __global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
   const int64_t col = (first >> a.page_shift) + ordinal;
   const int64_t lo = max(first, col << a.page_shift), hi = min(len, (col + 1) << a.page_shift);
   if (ordinal < 0 || n <= 0 || lo >= hi || col >= a.width) return;
-  const int32_t id = a.table[(int64_t)b * a.table_stride + col];
-  if (id < 0 || id >= a.pages) return;
   const int64_t src0 = row0 + (lo - start);                   // the first row of k / v for this page
   const int t0 = (int)(lo & (page - 1)), m = (int)(hi - lo);
   if (src0 < 0 || src0 + m > a.rows) return;
-  if (threadIdx.x < 2) s_mag[threadIdx.x] = 0;
+  const int vec_shift = __builtin_ctz((unsigned)a.dim) - 3, vecs = m << vec_shift;   // 16-byte pieces of the rows
+  const int64_t row = is_v ? a.v_row : a.k_row;
+  const uint16_t* src = (is_v ? a.v + head * a.v_head : a.k + head * a.k_head) + src0 * row;
+  auto piece = [&](int i) {
+    return *reinterpret_cast<const uint4*>(src + (i >> vec_shift) * row + (i & ((1 << vec_shift) - 1)) * 8);
+  };
+  uint4 keep[kKeep];
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) {
+    keep[j] = uint4{0, 0, 0, 0};
+    if (tid + T * j < vecs) keep[j] = piece(tid + T * j);
+  }
+  const int32_t id = a.table[(int64_t)b * a.table_stride + col];
+  if (tid == 0) s_mag = 0;
   __syncthreads();
+  if (id < 0 || id >= a.pages) return;
 
-  const int vecs = a.dim / 8;         // 16-byte pieces of a row
-  const uint16_t* ks = a.k + src0 * a.k_row + head * a.k_head;
-  const uint16_t* vs = a.v + src0 * a.v_row + head * a.v_head;
   auto largest = [](uint4 w, uint32_t mag) {
     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -125,82 +140,72 @@ __global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
     }
     return mag;
   };
-  uint32_t km = 0, vm = 0;
-  for (int i = (int)threadIdx.x; i < m * vecs; i += T) {
-    const int r = i / vecs, d = i % vecs * 8;
-    km = largest(*reinterpret_cast<const uint4*>(ks + r * a.k_row + d), km);
-    vm = largest(*reinterpret_cast<const uint4*>(vs + r * a.v_row + d), vm);
-  }
+  uint8_t* exp = (is_v ? a.ve : a.ke) + id * a.exp_page_stride + head * a.exp_head_stride;
+  const int e0 = t0 > 0 ? *exp : 0;                           // a page that takes its first row starts anew
+  uint32_t mag = 0;
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) {
-    km = max(km, (uint32_t)__shfl_xor((int)km, s));
-    vm = max(vm, (uint32_t)__shfl_xor((int)vm, s));
+  for (int j = 0; j < kKeep; ++j) mag = largest(keep[j], mag);
+  for (int i = tid + T * kKeep; i < vecs; i += T) mag = largest(piece(i), mag);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, d));
+  if (T > 64) {
+    if ((tid & 63) == 0) atomicMax(&s_mag, mag);
+    __syncthreads();
+    mag = s_mag;
   }
-  if ((threadIdx.x & 63) == 0) {
-    atomicMax(&s_mag[0], km);
-    atomicMax(&s_mag[1], vm);
-  }
-  uint8_t* ke = a.ke + id * a.exp_page_stride + head * a.exp_head_stride;
-  uint8_t* ve = a.ve + id * a.exp_page_stride + head * a.exp_head_stride;
-  // a page that takes its first row starts anew
-  const int ke0 = t0 > 0 ? *ke : 0, ve0 = t0 > 0 ? *ve : 0;
-  __syncthreads();
-  const int ke1 = max(ke0, scale_exponent(s_mag[0])), ve1 = max(ve0, scale_exponent(s_mag[1]));
-  const float kmul = exp_bits(254 - ke1), vmul = exp_bits(254 - ve1);   // 2^(127 - e)
-  uint8_t* kp = a.kp + id * a.page_stride + head * a.head_stride;
-  uint8_t* vp = a.vp + id * a.page_stride + head * a.head_stride;
+  const int e1 = max(e0, scale_exponent(mag));
+  const float mul = exp_bits(254 - e1);                       // 2^(127 - e)
+  uint8_t* out = (is_v ? a.vp : a.kp) + id * a.page_stride + head * a.head_stride;
 
   // the page's earlier rows, where the scale grew
-  if (t0 > 0 && ke1 > ke0) {
-    const float f = exp_bits(127 - (ke1 - ke0));
-    for (int i = (int)threadIdx.x; i < t0 * a.dim; i += T) {
-      const float x = e4m3_decode(kp[i]) * f;
-      kp[i] = (uint8_t)e4m3_pair(x, x);
-    }
-  }
-  if (t0 > 0 && ve1 > ve0) {
-    const float f = exp_bits(127 - (ve1 - ve0));
-    for (int i = (int)threadIdx.x; i < t0 * a.dim; i += T) {
-      uint8_t* p = vp + (i / t0 << a.page_shift) + i % t0;
+  if (t0 > 0 && e1 > e0) {
+    const float f = exp_bits(127 - (e1 - e0));
+    for (int i = tid; i < t0 * a.dim; i += T) {
+      uint8_t* p = is_v ? out + (i / t0 << a.page_shift) + i % t0 : out + i;
       const float x = e4m3_decode(*p) * f;
       *p = (uint8_t)e4m3_pair(x, x);
     }
   }
-  // the new rows: K as they lie, V through LDS
-  auto quantize = [](uint4 w, float mul) {
+  const int pitch = page + 4;
+  auto put = [&](int i, uint4 w) {
     uint2 q;
     q.x = e4m3_pair(bf16_bits_to_f32(w.x & 0xFFFFu) * mul, bf16_bits_to_f32(w.x >> 16) * mul) |
           e4m3_pair(bf16_bits_to_f32(w.y & 0xFFFFu) * mul, bf16_bits_to_f32(w.y >> 16) * mul) << 16;
     q.y = e4m3_pair(bf16_bits_to_f32(w.z & 0xFFFFu) * mul, bf16_bits_to_f32(w.z >> 16) * mul) |
           e4m3_pair(bf16_bits_to_f32(w.w & 0xFFFFu) * mul, bf16_bits_to_f32(w.w >> 16) * mul) << 16;
-    return q;
-  };
-  const int pitch = page + 4;
-  for (int i = (int)threadIdx.x; i < m * vecs; i += T) {
-    const int r = i / vecs, d = i % vecs * 8;
-    *reinterpret_cast<uint2*>(kp + (t0 + r) * a.dim + d) =
-        quantize(*reinterpret_cast<const uint4*>(ks + r * a.k_row + d), kmul);
-    const uint2 q = quantize(*reinterpret_cast<const uint4*>(vs + r * a.v_row + d), vmul);
+    const int r = i >> vec_shift, d = (i & ((1 << vec_shift) - 1)) * 8;
+    if (!is_v) {
+      *reinterpret_cast<uint2*>(out + (t0 + r) * a.dim + d) = q;
+    } else if (m == 1) {                                      // one byte of each dimension: straight to its place
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s_vt[(d + j) * pitch + t0 + r] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
-  }
-  __syncthreads();
-  if (t0 % 4 == 0 && m % 4 == 0) {
-    const int words = m / 4;
-    for (int i = (int)threadIdx.x; i < a.dim * words; i += T) {
-      const int d = i / words, t = t0 + i % words * 4;
-      *reinterpret_cast<uint32_t*>(vp + (d << a.page_shift) + t) = *reinterpret_cast<uint32_t*>(s_vt + d * pitch + t);
+      for (int j = 0; j < 8; ++j) out[((d + j) << a.page_shift) + t0] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s_vt[(d + j) * pitch + t0 + r] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
     }
-  } else {
-    for (int i = (int)threadIdx.x; i < a.dim * m; i += T) {
-      const int d = i / m, t = t0 + i % m;
-      vp[(d << a.page_shift) + t] = s_vt[d * pitch + t];
+  };
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (tid + T * j < vecs) put(tid + T * j, keep[j]);
+  for (int i = tid + T * kKeep; i < vecs; i += T) put(i, piece(i));
+  if (is_v && m > 1) {
+    __syncthreads();
+    // whole words of a dimension's row, and bytes at its ends
+    const int w0 = (t0 + 3) >> 2, w1 = (t0 + m) >> 2, words = w1 > w0 ? w1 - w0 : 0;
+    if (words > 0) {
+      for (int i = tid; i < a.dim * words; i += T) {
+        const int d = i / words, t = (w0 + i % words) * 4;
+        *reinterpret_cast<uint32_t*>(out + (d << a.page_shift) + t) = *reinterpret_cast<uint32_t*>(s_vt + d * pitch + t);
+      }
+    }
+    const int head_end = words > 0 ? w0 * 4 : t0 + m, tail = words > 0 ? w1 * 4 : t0 + m;
+    const int ends = (head_end - t0) + (t0 + m - tail);
+    for (int i = tid; i < a.dim * ends; i += T) {
+      const int d = i / ends, k = i % ends, t = k < head_end - t0 ? t0 + k : tail + k - (head_end - t0);
+      out[(d << a.page_shift) + t] = s_vt[d * pitch + t];
     }
   }
-  if (threadIdx.x == 0) {
-    *ke = (uint8_t)ke1;
-    *ve = (uint8_t)ve1;
-  }
+  if (tid == 0) *exp = (uint8_t)e1;
 }
 
 // --- attention: the work and its division ------------------------------------------------------------------------------
@@ -302,15 +307,7 @@ __device__ inline Entry entry_at(const AttnArgs& a, int e, int m_rows) {
 template <int T>
 __device__ inline void block_sums(int x, int y, int* s, int* x_before, int* x_all, int* y_before, int* y_all) {
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  int xi = x, yi = y;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(xi, d), v = __shfl_up(yi, d);
-    if (lane >= d) {
-      xi += u;
-      yi += v;
-    }
-  }
+  const int xi = wave_inclusive_sum(x), yi = wave_inclusive_sum(y);
   __syncthreads();
   if (lane == 63) {
     s[wave] = xi;
@@ -370,24 +367,14 @@ __device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
     // an entry to a lane, every wave by itself: no barriers (1 request of 4099 keys, 18.5 us with them, 17.3 without)
     const int lane = (int)threadIdx.x & 63;
     const int tiles = lane < a.entries ? entry_at(a, lane, m_rows).tiles : 0;
-    int all = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    const int all = __builtin_amdgcn_readlane(wave_inclusive_sum(tiles), 63);
     const int n_live = __popcll(__ballot(tiles > 0)), sure = max(max(room - n_live, room / 2), 1);
     const int least = least_piece(a, m_rows, all, n_live);
     int size = max((all + room - 1) / room, least), n, upto, cut;
     for (int tries = 0;; ++tries) {
       n = (tiles + size - 1) / size;
-      upto = n;
-      cut = n > 1 ? n : 0;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(upto, d), v = __shfl_up(cut, d);
-        if (lane >= d) {
-          upto += u;
-          cut += v;
-        }
-      }
+      upto = wave_inclusive_sum(n);
+      cut = wave_inclusive_sum(n > 1 ? n : 0);
       if (__builtin_amdgcn_readlane(upto, 63) <= room || tries == 1) break;
       size = max((all + sure - 1) / sure, least);
     }
@@ -1735,7 +1722,7 @@ extern "C" int xt_page8_append(const void* k, int64_t k_row_stride, int64_t k_he
                k_pages, vt_pages, k_exp, v_exp, page_stride, head_stride, exp_page_stride, exp_head_stride, pages,
                page_shift_of(page_size), kv_heads, dim, table, table_stride, width, seq_lens, cu_rows, batch};
   const int64_t units = cu_rows ? rows / page_size + 2 * (int64_t)batch : batch;
-  const dim3 grid((unsigned)units, kv_heads);
+  const dim3 grid((unsigned)units, kv_heads, 2);
   const size_t lds = (size_t)dim * (page_size + 4);
   if (!cu_rows) append_kernel<64><<<grid, 64, lds, stream>>>(a);
   else append_kernel<256><<<grid, 256, lds, stream>>>(a);

@@ -14,27 +14,23 @@ namespace {
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / 64;
 
-// Exclusive prefix of x over the workgroup's threads, and the total. `s` holds kScanWaves + 1 values of the caller.
-__device__ inline int64_t block_exclusive(int64_t x, int64_t* s, int64_t* total) {
+// Sums of x over the workgroup's threads before this one, and over all (both below 2^31). `s` holds kScanWaves values of
+// the caller.
+__device__ inline int block_exclusive(int x, int* s, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t incl = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(incl, d);
-    if (lane >= d) incl += y;
-  }
+  const int upto = wave_inclusive_sum(x);
   __syncthreads();                       // earlier readers of s are done
-  if (lane == 63) s[wave] = incl;
+  if (lane == 63) s[wave] = upto;
   __syncthreads();
-  int64_t before = 0, all = 0;
+  int before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kScanWaves; ++w) {
-    const int64_t v = s[w];
+    const int v = s[w];
     if (w < wave) before += v;
     all += v;
   }
   *total = all;
-  return before + incl - x;
+  return before + upto - x;
 }
 
 // The pages of this thread: [lo, hi), spans of a multiple of 4 pages.
@@ -45,8 +41,8 @@ __device__ inline void span_of(int64_t pages, int64_t* lo, int64_t* hi) {
   *hi = l + per < pages ? l + per : pages;
 }
 
-__device__ inline int64_t count_free(const int32_t* refs, int64_t lo, int64_t hi) {
-  int64_t n = 0;
+__device__ inline int count_free(const int32_t* refs, int64_t lo, int64_t hi) {
+  int n = 0;
   for (int64_t p = lo; p < hi; ++p) n += refs[p] == 0;
   return n;
 }
@@ -57,17 +53,18 @@ __global__ __launch_bounds__(kScanThreads) void extend_kernel(int32_t* refs, int
                                                                const int32_t* add, int rows, int page_shift,
                                                                uint8_t* granted, int32_t* free_list,
                                                                int64_t free_cap) {
-  __shared__ int64_t s[kScanWaves + 1];
-  int64_t lo, hi, n_free;
+  __shared__ int s[kScanWaves];
+  int64_t lo, hi;
+  int n_free;
   span_of(pages, &lo, &hi);
-  const int64_t mine = count_free(refs, lo, hi);
+  const int mine = count_free(refs, lo, hi);
   int64_t rank = block_exclusive(mine, s, &n_free);
   // the free list, as far as any row may need it (free_cap entries): rank -> page
   for (int64_t p = lo; p < hi && rank < free_cap; ++p)
     if (refs[p] == 0) free_list[rank++] = (int32_t)p;
   __syncthreads();   // the list is written and every count of refs == 0 is read before any refs changes
   const int64_t mask = (1 << page_shift) - 1;
-  __shared__ int64_t s_upto[kScanThreads];     // pages needed by this round's rows up to and with this one
+  __shared__ int s_upto[kScanThreads];         // pages needed by this round's rows up to and with this one
   __shared__ int32_t s_col[kScanThreads];      // the first new column of a granted row, -1 for one that gets none
   int64_t base = 0;                            // pages needed by the rows of earlier rounds
   for (int r0 = 0; r0 < rows; r0 += kScanThreads) {
@@ -81,9 +78,9 @@ __global__ __launch_bounds__(kScanThreads) void extend_kernel(int32_t* refs, int
       c1 = (len + grow + mask) >> page_shift;
       fits = len >= 0 && grow >= 0 && c1 <= width && len + grow <= 0x7FFFFFFF;
     }
-    const int64_t need = fits ? c1 - c0 : 0;
-    int64_t round;
-    const int64_t from = block_exclusive(need, s, &round);
+    const int need = fits ? (int)(c1 - c0) : 0;    // (1024 rows of at most 2^21 - 1 columns, which the host sees to)
+    int round;
+    const int from = block_exclusive(need, s, &round);
     const bool granted_here = fits && (need == 0 || base + from + need <= n_free);
     s_upto[threadIdx.x] = from + need;
     s_col[threadIdx.x] = granted_here ? (int32_t)c0 : -1;
@@ -93,7 +90,7 @@ __global__ __launch_bounds__(kScanThreads) void extend_kernel(int32_t* refs, int
     }
     __syncthreads();
     // one thread a page, whichever row it belongs to: the first whose running need passes it
-    for (int64_t j = threadIdx.x; j < round && base + j < n_free; j += kScanThreads) {
+    for (int j = (int)threadIdx.x; j < round && base + j < n_free; j += kScanThreads) {
       int at = 0;
 #pragma unroll
       for (int step = kScanThreads / 2; step > 0; step >>= 1)
@@ -108,67 +105,87 @@ __global__ __launch_bounds__(kScanThreads) void extend_kernel(int32_t* refs, int
   }
 }
 
-// Fork plan: checks each fork, finds its page for the unfinished one, writes its moves and lengths, and leaves per fork
-// {parent row or -1, pages shared, destination page or -1} in `plan` for fork_rows_kernel. One workgroup.
-__global__ __launch_bounds__(kScanThreads) void fork_plan_kernel(int32_t* refs, int64_t pages, const int32_t* table,
-                                                                  int64_t table_stride, int width, int32_t* lens,
-                                                                  int rows, int page_shift, const int32_t* parents,
-                                                                  const int32_t* children, int n, int32_t* moves,
-                                                                  int64_t moves_stride, int32_t* plan,
-                                                                  int32_t* free_list) {
-  __shared__ int64_t s[kScanWaves + 1];
-  __shared__ int32_t s_child[kScanThreads];
-  int64_t lo, hi, n_free, n_need;
+// One column of a child's row: the parent's full pages, which gain a reference, then the new page, then none.
+__device__ inline void fork_cell(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int c,
+                                 int32_t parent, int32_t child, int32_t full, int32_t dst) {
+  int32_t p = -1;
+  if (c < full) {
+    p = table[(int64_t)parent * table_stride + c];
+    if (p >= 0 && p < pages) atomicAdd(&refs[p], 1);
+  } else if (c == full) {
+    p = dst;
+  }
+  table[(int64_t)child * table_stride + c] = p;
+}
+
+// Checks each fork, finds its page for the unfinished one and writes its moves and lengths. Then the children's rows, if
+// `plan` is NULL; else per fork {parent row or -1, pages shared, destination page or -1} for fork_rows_kernel. One
+// workgroup: up to XT_PAGES_FORK_CELLS columns a second launch costs more than it gains (32 forks of 66 columns: 34 us with
+// the copy of 12 layers and the rest of a step, 31 in one).
+__global__ __launch_bounds__(kScanThreads) void fork_kernel(int32_t* refs, int64_t pages, int32_t* table,
+                                                             int64_t table_stride, int width, int32_t* lens, int rows,
+                                                             int page_shift, const int32_t* parents,
+                                                             const int32_t* children, int n, int32_t* moves,
+                                                             int64_t moves_stride, int32_t* plan) {
+  __shared__ int s[kScanWaves];
+  __shared__ int32_t s_child[kScanThreads], s_free[kScanThreads], s_plan[3][kScanThreads];
+  int64_t lo, hi;
+  int n_free, n_need;
   span_of(pages, &lo, &hi);
   const int i = (int)threadIdx.x;
   const bool mine = i < n;
   const int32_t parent = mine ? parents[i] : -1, child = mine ? children[i] : -1;
   s_child[i] = child;
-  const int64_t n_mine = count_free(refs, lo, hi);
-  int64_t rank = block_exclusive(n_mine, s, &n_free);
-  for (int64_t p = lo; p < hi && rank < n; ++p)
-    if (refs[p] == 0) free_list[rank++] = (int32_t)p;
   bool ok = mine && parent >= 0 && parent < rows && child >= 0 && child < rows;
   int64_t len = 0;
   if (ok) {
     len = lens[parent] > 0 ? lens[parent] : 0;
     ok = lens[child] == 0;
   }
+  const int n_mine = count_free(refs, lo, hi);
+  int rank = block_exclusive(n_mine, s, &n_free);
+  for (int64_t p = lo; p < hi && rank < n; ++p)
+    if (refs[p] == 0) s_free[rank++] = (int32_t)p;
   for (int j = 0; j < i && ok; ++j) ok = s_child[j] != child;   // a child takes its first fork
   const int64_t full = len >> page_shift;
   const bool need = ok && (len & ((1 << page_shift) - 1)) != 0;
-  const int64_t at = block_exclusive(need ? 1 : 0, s, &n_need);   // (its barriers: every lens is read before any is written)
-  if (!mine) return;
-  const int32_t dst = need && at < n_free && full < width ? free_list[at] : -1;
-  int32_t src = dst >= 0 ? table[(int64_t)parent * table_stride + full] : -1;
-  moves[i] = src;
-  moves[moves_stride + i] = dst;
-  if (ok) lens[child] = (int32_t)(need && dst < 0 ? full << page_shift : len);
-  if (dst >= 0) refs[dst] = 1;
-  plan[3 * i] = ok ? parent : -1;
-  plan[3 * i + 1] = (int32_t)(full < width ? full : width);
-  plan[3 * i + 2] = dst;
+  const int at = block_exclusive(need ? 1 : 0, s, &n_need);   // (its barriers: every lens is read before any is written)
+  const int32_t dst = need && at < n_free && full < width ? s_free[at] : -1;
+  if (mine) {
+    moves[i] = dst >= 0 ? table[(int64_t)parent * table_stride + full] : -1;
+    moves[moves_stride + i] = dst;
+    if (ok) lens[child] = (int32_t)(need && dst < 0 ? full << page_shift : len);
+    if (dst >= 0) refs[dst] = 1;
+  }
+  const int32_t shared = (int32_t)(full < width ? full : width);
+  if (plan) {
+    if (mine) {
+      plan[3 * i] = ok ? parent : -1;
+      plan[3 * i + 1] = shared;
+      plan[3 * i + 2] = dst;
+    }
+    return;
+  }
+  s_plan[0][i] = ok ? parent : -1;
+  s_plan[1][i] = shared;
+  s_plan[2][i] = dst;
+  __syncthreads();
+  // (a row that is both a parent and a child held no tokens: none of its columns is read)
+  for (int k = i; k < n * width; k += kScanThreads) {
+    const int f = k / width;
+    if (s_plan[0][f] >= 0)
+      fork_cell(refs, pages, table, table_stride, k % width, s_plan[0][f], s_child[f], s_plan[1][f], s_plan[2][f]);
+  }
 }
 
-// The table rows of the children: the parent's full pages, then the new page, then none. grid (n, column chunks).
+// The table rows of the children. grid (n, column chunks).
 __global__ __launch_bounds__(256) void fork_rows_kernel(int32_t* refs, int64_t pages, int32_t* table,
                                                          int64_t table_stride, int width, const int32_t* children,
                                                          const int32_t* plan) {
   const int i = (int)blockIdx.x;
-  const int32_t parent = plan[3 * i];
-  if (parent < 0) return;
-  const int32_t full = plan[3 * i + 1], dst = plan[3 * i + 2];
-  const int64_t child = children[i];
-  for (int c = (int)(blockIdx.y * 256 + threadIdx.x); c < width; c += (int)gridDim.y * 256) {
-    int32_t p = -1;
-    if (c < full) {
-      p = table[(int64_t)parent * table_stride + c];
-      if (p >= 0 && p < pages) atomicAdd(&refs[p], 1);
-    } else if (c == full) {
-      p = dst;
-    }
-    table[child * table_stride + c] = p;
-  }
+  if (plan[3 * i] < 0) return;
+  for (int c = (int)(blockIdx.y * 256 + threadIdx.x); c < width; c += (int)gridDim.y * 256)
+    fork_cell(refs, pages, table, table_stride, c, plan[3 * i], children[i], plan[3 * i + 1], plan[3 * i + 2]);
 }
 
 // grid (n, column chunks): each entry of the row is taken by one thread (the exchange), whose count it gives back, so
@@ -188,19 +205,17 @@ __global__ __launch_bounds__(256) void free_kernel(int32_t* refs, int64_t pages,
 // in use) where it is afterwards: map[page]. One workgroup.
 __global__ __launch_bounds__(kScanThreads) void compact_plan_kernel(int32_t* refs, int64_t pages, int32_t* moves,
                                                                      int64_t half, int32_t* count, int32_t* map) {
-  __shared__ int64_t s[kScanWaves + 1];
-  int64_t lo, hi, live, n_src, n_dst;
+  __shared__ int s[kScanWaves];
+  int64_t lo, hi;
+  int live, n_src;
   span_of(pages, &lo, &hi);
-  int64_t used = 0;
+  int used = 0;
   for (int64_t p = lo; p < hi; ++p) used += refs[p] > 0;
-  block_exclusive(used, s, &live);
-  int64_t src = 0, dst = 0;
-  for (int64_t p = lo; p < hi; ++p) {
-    const bool u = refs[p] > 0;
-    src += u && p >= live;
-    dst += !u && p < live;
-  }
-  int64_t rs = block_exclusive(src, s, &n_src), rd = block_exclusive(dst, s, &n_dst);
+  const int used_before = block_exclusive(used, s, &live);
+  // pages of this span in use at or above the mark, and free below it; those before the span follow from `used_before`
+  int src = 0;
+  for (int64_t p = max(lo, (int64_t)live); p < hi; ++p) src += refs[p] > 0;
+  int64_t rs = block_exclusive(src, s, &n_src), rd = lo - used_before;
   for (int64_t p = lo; p < hi; ++p) {
     const bool u = refs[p] > 0;
     if (p >= live) {
@@ -210,7 +225,7 @@ __global__ __launch_bounds__(kScanThreads) void compact_plan_kernel(int32_t* ref
       moves[half + rd++] = (int32_t)p;
     }
   }
-  // n_src == n_dst <= pages / 2: as many pages in use lie above the mark as free ones below it
+  // n_src <= pages / 2: as many pages in use lie above the mark as free ones below it
   for (int64_t i = n_src + threadIdx.x; i < half; i += kScanThreads) moves[i] = moves[half + i] = -1;
   if (threadIdx.x == 0) *count = (int32_t)n_src;
   __syncthreads();
@@ -285,10 +300,7 @@ int column_chunks(int width) { return width > 4096 ? 4 : (width + 1023) / 1024; 
 
 using namespace xt;
 
-extern "C" size_t xt_pages_workspace_bytes(int64_t pages, int forks) {
-  if (pages < 0 || forks < 0) return 0;
-  return ((size_t)pages + 4 * (size_t)forks) * 4;
-}
+extern "C" size_t xt_pages_workspace_bytes(int64_t pages) { return pages < 0 ? 0 : (size_t)pages * 4; }
 
 extern "C" int xt_pages_extend(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width,
                                int32_t* lens, const int32_t* add, int rows, int page_size, uint8_t* granted,
@@ -299,9 +311,10 @@ extern "C" int xt_pages_extend(int32_t* refs, int64_t pages, int32_t* table, int
   const int shift = page_shift_of(page_size);
   if (!lens || !add || !granted || shift < 0)
     return fail(XT_EINVAL, "%s: null pointer or page size %d not a power of 2", what, page_size);
-  if (!workspace || workspace_bytes < xt_pages_workspace_bytes(pages, 0))
+  if (width > 0x1FFFFF) return fail(XT_EUNSUPPORTED, "%s: a table of %d columns", what, width);
+  if (!workspace || workspace_bytes < xt_pages_workspace_bytes(pages))
     return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes,
-                xt_pages_workspace_bytes(pages, 0));
+                xt_pages_workspace_bytes(pages));
   extend_kernel<<<1, kScanThreads, 0, stream>>>(refs, pages, table, table_stride, width, lens, add, rows, shift,
                                                 granted, (int32_t*)workspace, pages);
   return check_launch(what);
@@ -318,13 +331,15 @@ extern "C" int xt_pages_fork(int32_t* refs, int64_t pages, int32_t* table, int64
   if (forks < 0 || !lens || !parents || !children || !moves || moves_stride < forks || shift < 0)
     return fail(XT_EINVAL, "%s: null pointer, negative count or page size %d not a power of 2", what, page_size);
   if (forks > kScanThreads) return fail(XT_EUNSUPPORTED, "%s: %d forks in one call, at most %d", what, forks, kScanThreads);
-  if (!workspace || workspace_bytes < xt_pages_workspace_bytes(pages, forks))
-    return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes,
-                xt_pages_workspace_bytes(pages, forks));
-  int32_t* plan = (int32_t*)workspace;
-  fork_plan_kernel<<<1, kScanThreads, 0, stream>>>(refs, pages, table, table_stride, width, lens, rows, shift, parents,
-                                                   children, forks, moves, moves_stride, plan, plan + 3 * forks);
+  const bool small = (int64_t)forks * width <= XT_PAGES_FORK_CELLS;
+  const size_t need = small ? 0 : (size_t)forks * 12;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  int32_t* plan = small ? nullptr : (int32_t*)workspace;
+  fork_kernel<<<1, kScanThreads, 0, stream>>>(refs, pages, table, table_stride, width, lens, rows, shift, parents,
+                                              children, forks, moves, moves_stride, plan);
   if (const int st = check_launch(what)) return st;
+  if (small) return ok();
   fork_rows_kernel<<<dim3(forks, column_chunks(width)), 256, 0, stream>>>(refs, pages, table, table_stride, width,
                                                                           children, plan);
   return check_launch(what);
@@ -347,9 +362,9 @@ extern "C" int xt_pages_compact(int32_t* refs, int64_t pages, int32_t* table, in
   const char* what = "xt_pages_compact";
   if (const int st = check_table(what, refs, pages, table, table_stride, width, rows)) return st;
   if ((!moves && pages > 1) || !count) return fail(XT_EINVAL, "%s: null pointer", what);
-  if (!workspace || workspace_bytes < xt_pages_workspace_bytes(pages, 0))
+  if (!workspace || workspace_bytes < xt_pages_workspace_bytes(pages))
     return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes,
-                xt_pages_workspace_bytes(pages, 0));
+                xt_pages_workspace_bytes(pages));
   int32_t* map = (int32_t*)workspace;
   const int64_t half = pages / 2;
   compact_plan_kernel<<<1, kScanThreads, 0, stream>>>(refs, pages, moves, half, count, map);

@@ -118,6 +118,17 @@ __device__ inline float sum4_lanes16(float x) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+// Inclusive sums of x over the wave's lanes, by data-parallel moves between lanes (row shifts within 16 lanes, then the
+// last lane of a row and of the lower half broadcast): no LDS round trips, as __shfl_up has.
+__device__ inline int wave_inclusive_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
+  return x;
+}
 // The power of two 2^e that brings a head's largest query magnitude `qmax` into [2^10, 2^11): the query enters FP16
 // MFMA operands as q * 2^-e, exactly for every element down to 2^-24 of qmax (BF16's 8 significant bits fit FP16's
 // 11 within its normal range; smaller elements weigh less than that in any score), and 2^e multiplies the FP32
@@ -180,6 +191,7 @@ __device__ inline void reset_counter(int32_t* counter) {
 }
 #else
 // The host pass parses device code without the gfx950 builtins; these declarations are never code-generated.
+__device__ int wave_inclusive_sum(int x);
 __device__ float2_t pow2_query_scale(float qmax);
 __device__ void store_partial(__amdgpu_buffer_rsrc_t r, int byte_off, float4_t v);
 __device__ float4_t load_partial(__amdgpu_buffer_rsrc_t r, int byte_off);

@@ -1282,8 +1282,8 @@ def _check_pages(what, refs, table, lens=None):
     return refs.shape[0], table.stride(0), table.shape[1], table.shape[0]
 
 
-def _pages_workspace(refs, forks=0):
-    return torch.empty(refs.shape[0] + 4 * forks, dtype=torch.int32, device=refs.device)
+def _pages_workspace(refs):
+    return torch.empty(refs.shape[0], dtype=torch.int32, device=refs.device)
 
 
 def pages_extend(refs, table, lens, add, page_size):
@@ -1320,10 +1320,11 @@ def pages_fork(refs, table, lens, parents, children, page_size):
             return pages_fork(refs, table, lens, parents, children, page_size)
     n = parents.shape[0]
     moves = torch.empty((2, n), dtype=torch.int32, device=refs.device)
-    ws, parents, children = _pages_workspace(refs, n), _int32(parents), _int32(children)
+    ws = torch.empty(3 * n, dtype=torch.int32, device=refs.device) if n * width > _lib.PAGES_FORK_CELLS else None
+    parents, children = _int32(parents), _int32(children)
     _lib.check(_lib.lib().xt_pages_fork(
         refs.data_ptr(), pages, table.data_ptr(), stride, width, lens.data_ptr(), rows, int(page_size),
-        parents.data_ptr(), children.data_ptr(), n, moves.data_ptr(), n, ws.data_ptr(), ws.shape[0] * 4,
+        parents.data_ptr(), children.data_ptr(), n, moves.data_ptr(), n, _ptr(ws), 12 * n if ws is not None else 0,
         _stream(refs)), 'pages_fork')
     return moves
 
