@@ -398,8 +398,9 @@ size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_heads, int 
  * q_heads / kv_heads <= 128; scale > 0; out: out_dtype (strides in elements, 8-byte aligned rows); lse (optional): FP32
  * [rows, q_heads]. QK exact products of BF16 with FP32 sums; P and V as FP16 in the second product (V exact within 15
  * binades of scale below the largest of the row's pages), FP32 sums.
- * workspace: xt_page8_attention_workspace_bytes bytes, 256-byte aligned, zero before its first use and left so where it
- * has to be; calls of any shape may share one, one at a time. One launch on `stream`, its work divided on the device,
+ * workspace: xt_page8_attention_workspace_bytes bytes, 256-byte aligned. It begins with the 64 KB of arrival counters that
+ * the other decode entry points have too, zero before the first use and left zero; calls of any shape may share one, one
+ * at a time. Tables of up to 2^30 tokens and kv_heads <= 8192. One launch on `stream`, its work divided on the device,
  * so that a captured launch follows the lengths of each replay. */
 int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
                        const uint8_t* vt_pages, const uint8_t* k_exp, const uint8_t* v_exp, int64_t pages, int kv_heads,

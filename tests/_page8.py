@@ -59,4 +59,35 @@ def attention_tolerance(ref, lse, spread, score, raw, keys, dim, eps):
     return tol, lse_tol
 
 
-__all__ = ['attention_tolerance', 'bf16', 'gpu_raw', 'page8', 'pool_bytes', 'table_for']
+def attention_on_gpu(q, raw, table, page, lens, scale, cu, window=0, sinks=0):
+    """The same definition as oracle.page8.attention in plain float64 torch operations on the GPU, for sizes that are too
+    long on the CPU: (out, lse, spread, score) as numpy arrays. Every page is taken to exist."""
+    k8, vt8, ke, ve = (torch.from_numpy(x).cuda() for x in raw)
+    two_to = lambda e: ((e.long() - 127 + 1023) << 52).view(torch.float64)
+    q = q.cuda().double()
+    group = q.shape[1] // k8.shape[1]
+    out, spread = torch.empty_like(q), torch.empty_like(q)
+    lse, score = (torch.empty(q.shape[:2], dtype=torch.float64, device='cuda') for _ in range(2))
+    for b, length in enumerate(lens.tolist()):
+        lo, hi = int(cu[b]), int(cu[b + 1])
+        ids = torch.from_numpy(table[b, :-(-length // page)].astype(np.int64)).cuda()
+        p = torch.arange(length - (hi - lo), length, device='cuda')
+        for h in range(k8.shape[1]):
+            k = (k8[ids, h].view(torch.float8_e4m3fn).double() * two_to(ke[ids, h])[:, None, None]).flatten(0, 1)[:length]
+            v = (vt8[ids, h].view(torch.float8_e4m3fn).double() * two_to(ve[ids, h])[:, None, None])
+            v = v.transpose(1, 2).flatten(0, 1)[:length].contiguous()
+            j = torch.arange(length, device='cuda')
+            seen = j <= p[:, None]
+            if window:
+                seen &= (j > p[:, None] - window) | (j < sinks)
+            for g in range(h * group, (h + 1) * group):
+                qq = q[lo:hi, g]
+                z = (qq @ k.t() * scale).masked_fill(~seen, -np.inf)
+                lse[lo:hi, g] = torch.logsumexp(z, 1)
+                w = torch.exp(z - lse[lo:hi, g, None])
+                out[lo:hi, g], spread[lo:hi, g] = w @ v, w @ v.abs()
+                score[lo:hi, g] = (qq.abs() @ k.abs().t()).masked_fill(~seen, 0).amax(1) * scale
+    return tuple(x.cpu().numpy() for x in (out, lse, spread, score))
+
+
+__all__ = ['attention_on_gpu', 'attention_tolerance', 'bf16', 'gpu_raw', 'page8', 'pool_bytes', 'table_for']

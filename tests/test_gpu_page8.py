@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests._page8 import attention_tolerance, bf16, gpu_raw, page8, pool_bytes, table_for
+from tests._page8 import attention_on_gpu, attention_tolerance, bf16, gpu_raw, page8, pool_bytes, table_for
 from xtier_amd import ops
 from xtier_amd.pool import Page8Pool
 
@@ -126,9 +126,13 @@ def _attention_case(rng, lens, rows, page, heads, group, dim, q_std=1.0, spread=
 
 
 def _check_attention(raw, table, lens, cu, q, page, window=0, sinks=0, scale=0.01, pass_cu=True, out_dtype=None,
-                     pool=None):
+                     pool=None, large=False):
     pool = pool or gpu_raw(raw)
-    ref, ref_lse, spread, score = page8.attention(q.double().numpy(), raw, table, page, lens, scale, cu, window, sinks)
+    if large:
+        ref, ref_lse, spread, score = attention_on_gpu(q, raw, table, page, lens, scale, cu, window, sinks)
+    else:
+        ref, ref_lse, spread, score = page8.attention(q.double().numpy(), raw, table, page, lens, scale, cu, window,
+                                                      sinks)
     lse = torch.full(q.shape[:2], 7.0, dtype=torch.float32, device='cuda')
     out = None if out_dtype is None else torch.empty(q.shape, dtype=out_dtype, device='cuda')
     out = pool.attend(q.cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(), scale,
@@ -275,6 +279,88 @@ def test_layouts_and_outputs():
     tol, _ = attention_tolerance(ref, np.zeros((5, 6)), spread, score, raw, 90, 128, 2.0 ** -7)
     assert (np.abs(got[:5].double().cpu().numpy() - ref) <= tol).all()
     assert (out[5:] == 5).all() and (out[:, :6] == 5).all() and (lse[5:] == 5).all() and (lse[:5] != 5).all()
+
+
+@pytest.mark.parametrize('dim,page', [(64, 16), (64, 128), (128, 32), (128, 64), (256, 16), (256, 64)])
+def test_prompt_chunks(dim, page):
+    """Many rows a request at every head size, small and large pages, beside requests with few rows and none; windows."""
+    rng = np.random.default_rng(dim + page)
+    lens, rows = [333, 64, 90, 500, 201], [300, 64, 0, 77, 201]
+    case = _attention_case(rng, lens, rows, page, 2, 3, dim)
+    _check_attention(*case, page, large=True)
+    _check_attention(*case, page, window=70, sinks=3, large=True)
+    _check_attention(*case, page, window=200, sinks=130, large=True)
+
+
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_nan_in_prompt_chunks(dim):
+    """A NaN value that some rows of a tile see and others do not; stale NaN bytes behind the last token."""
+    rng = np.random.default_rng(dim)
+    for page in (16, 64):
+        raw, table, lens, cu, q = _attention_case(rng, [230], [100], page, 1, 4, dim)
+        raw[1][table[0, 190 // page], 0, 7, 190 % page] = 0x7F
+        raw[1][table[0, 140 // page], 0, dim - 1, 140 % page] = 0xFF
+        raw[0][table[0, 229 // page], 0, 229 % page + 1:] = 0x7F
+        raw[1][table[0, 229 // page], 0, :, 229 % page + 1:] = 0x7F
+        _check_attention(raw, table, lens, cu, q, page)
+        _check_attention(raw, table, lens, cu, q, page, window=60, sinks=2)
+
+
+def test_many_prompts():
+    """More entries than workgroups: whole entries in rounds, and runs across entries."""
+    rng = np.random.default_rng(31)
+    for lens, rows, heads in (([900] * 9, [700] * 9, 4), ([2100] * 5, [2000] * 5, 4)):
+        _check_attention(*_attention_case(rng, lens, rows, 64, heads, 4, 64), 64, large=True)
+    _check_attention(*_attention_case(rng, [1500] * 7, [1000] * 7, 64, 4, 2, 128), 64, window=300, sinks=4, large=True)
+
+
+def test_a_long_prompt_cut_into_pieces():
+    rng = np.random.default_rng(32)
+    for dim, group in ((64, 4), (128, 8), (256, 2)):
+        _check_attention(*_attention_case(rng, [9000], [100], 64, 1, group, dim), 64, large=True)
+        _check_attention(*_attention_case(rng, [6000, 40], [9, 9], 32, 2, 5, dim), 32, large=True)
+
+
+def test_many_requests():
+    """More entries than lanes of a wave and threads of a workgroup, with and without row offsets, one of them long."""
+    rng = np.random.default_rng(33)
+    for n in (65, 300):
+        lens = (rng.integers(1, 90, n)).tolist()
+        lens[n // 2] = 4000
+        _check_attention(*_attention_case(rng, lens, [1] * n, 16, 1, 4, 64), 16, pass_cu=False, large=True)
+        _check_attention(*_attention_case(rng, lens, rng.integers(0, 2, n).tolist(), 16, 1, 4, 64), 16, large=True)
+    lens = rng.integers(40, 90, 130).tolist()
+    _check_attention(*_attention_case(rng, lens, [40] * 130, 16, 1, 4, 64), 16, large=True)
+
+
+def test_calls_of_differing_shapes_share_a_workspace():
+    """Calls whose partials lie at different places, one after the other in one workspace: each finds its counters zero."""
+    rng = np.random.default_rng(34)
+    cases = [_attention_case(rng, [5000], [100], 64, 1, 8, 128), _attention_case(rng, [4000, 100], [1, 1], 64, 1, 8, 64),
+             _attention_case(rng, [3000], [200], 64, 2, 4, 64), _attention_case(rng, [6000], [1], 64, 4, 2, 256),
+             _attention_case(rng, [5000, 3000], [4, 4], 64, 2, 8, 128)]
+    pools = [gpu_raw(c[0]) for c in cases]
+    ws = torch.zeros(128 << 20, dtype=torch.uint8, device='cuda')
+
+    def run(i, w):
+        raw, table, lens, cu, q = cases[i]
+        return pools[i].attend(q.cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(), 0.02,
+                               torch.from_numpy(cu).cuda(), ws=w)
+
+    alone = [run(i, torch.zeros(128 << 20, dtype=torch.uint8, device='cuda')) for i in range(len(cases))]
+    for i in (0, 1, 2, 3, 4, 2, 1, 0, 3, 4, 1):
+        assert torch.equal(run(i, ws), alone[i])
+        assert (ws[:65536] == 0).all()
+
+
+def test_wide_windows_are_no_windows():
+    rng = np.random.default_rng(35)
+    raw, table, lens, cu, q = _attention_case(rng, [300, 70], [20, 1], 32, 1, 4, 64)
+    pool = gpu_raw(raw)
+    args = (q.cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(), 0.02, torch.from_numpy(cu).cuda())
+    want = pool.attend(*args)
+    for window, sinks in ((300, 0), (1 << 30, 5), ((1 << 31) - 1, 1 << 40), (1 << 50, 0)):
+        assert torch.equal(pool.attend(*args, window=window, sinks=sinks), want)
 
 
 def test_same_result_every_time():

@@ -53,6 +53,8 @@ def test_attention(lib):
                 dict(scale=float('inf')), dict(scale=float('nan')), dict(out_dtype=2)):
         assert _attend(lib, **bad) == _lib.XT_EINVAL, bad
     assert _attend(lib, q_heads=129, heads=1) == _lib.XT_EUNSUPPORTED
+    for bad in (dict(width=1 << 25, ts=1 << 25), dict(heads=8200, q_heads=8200, rows=2), dict(ps=1 << 33)):
+        assert _attend(lib, **{'rows': 2, 'batch': 2, **bad}) == _lib.XT_EUNSUPPORTED, bad
     for bad in (dict(q=None), dict(q=P + 8), dict(q_rs=4097), dict(out=P + 4), dict(o_hs=126), dict(width=0),
                 dict(ts=1), dict(rows=3)):
         assert _attend(lib, **{'rows': 2, 'batch': 2, **bad}) == _lib.XT_EINVAL, bad
@@ -129,7 +131,9 @@ def test_python_checks():
             pool.attend(q, t, s, 0.1, cu)
     k, vt, ke, ve = pool.raw
     for raw in ((k.float(), vt, ke, ve), (k, k, ke, ve), (k, vt, ke[:4], ve), (k, vt, ke, ve.int()),
-                (k[:, :, ::2], vt, ke, ve), (k.contiguous(), vt, ke, ve), (k[0], vt, ke, ve)):
+                (k[:, :, ::2], vt, ke, ve), (k.contiguous(), vt, ke, ve), (k[0], vt, ke, ve),
+                (k[:1].expand(8, -1, -1, -1), vt[:1].expand(8, -1, -1, -1), ke, ve),
+                (k, vt, ke[:1].expand(8, -1), ve[:1].expand(8, -1))):
         with pytest.raises(ValueError, match='expected'):
             ops.page8_append(x, x, raw, table, lens)
     for page, dim in ((8, 64), (64, 96), (256, 128)):
@@ -152,6 +156,8 @@ def test_python_checks():
         ops.PageBuffers([torch.zeros(4, 6, 6)[:, :, :3]])
     with pytest.raises(ValueError, match='int32 moves'):
         ops.pages_copy([torch.zeros(4, 6)], torch.zeros(2, 3))
+    with pytest.raises(ValueError, match='int32 count'):
+        ops.pages_copy([torch.zeros(4, 6)], torch.zeros(2, 3, dtype=torch.int32), torch.zeros(0, dtype=torch.int32))
     with pytest.raises(ValueError, match='whole pages'):
         KVPool(40, 1, 64, device='cpu').page_buffers(16)
     assert [b.shape for b in LatentPool(32, device='cpu').page_buffers(16)] == [(2, 16 * 416)]

@@ -54,6 +54,7 @@ _CP, _KP, _FP = ctypes.POINTER(MlaCache), ctypes.POINTER(MlaKeys), ctypes.POINTE
 _SP = ctypes.POINTER(KvStore)
 _BP = ctypes.POINTER(PageBuffer)
 PAGES_COPY_MAX, PAGES_FORK_CELLS = 64, 16384
+COUNTER_BYTES = 65536      # the arrival counters at the start of every workspace
 
 SIGNATURES = {
     'xt_version': (_I, []),

@@ -1660,7 +1660,9 @@ Launch plan_launch(int rows, int batch, int heads, int group, int dim, bool ragg
   return x;
 }
 
-size_t counter_bytes(const Launch& x) { return ((size_t)x.partials * 4 + 255) / 256 * 256; }
+// The workspace: the fixed region of arrival counters (one per partial; at the same place for every shape, so that calls of
+// any shape may share it), then the partials.
+size_t attention_bytes(const Launch& x, int dim) { return kCounterBytes + (size_t)x.partials * x.m * (dim + 4) * 4; }
 
 }  // namespace
 }  // namespace xt
@@ -1733,10 +1735,8 @@ extern "C" size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_
   if (rows < 0 || batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || dim < 1 ||
       (int64_t)rows * (q_heads / kv_heads) > kMaxRows || (int64_t)batch * q_heads > kMaxRows)
     return 0;
-  const Launch x = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, dim, true);
-  const Launch y = plan_launch(rows, batch, kv_heads, q_heads / kv_heads, dim, false);
-  const size_t partial = (size_t)x.m * (dim + 4) * 4;
-  const size_t a = counter_bytes(x) + x.partials * partial, b = counter_bytes(y) + y.partials * partial;
+  const size_t a = attention_bytes(plan_launch(rows, batch, kv_heads, q_heads / kv_heads, dim, true), dim);
+  const size_t b = attention_bytes(plan_launch(rows, batch, kv_heads, q_heads / kv_heads, dim, false), dim);
   return a > b ? a : b;
 }
 
@@ -1793,10 +1793,18 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
       out_row_stride % 4 || out_head_stride % 4)
     return fail(XT_EINVAL, "%s: query rows must be 16-byte aligned, output rows 8-byte aligned", what);
   const Launch x = plan_launch(rows, batch, kv_heads, group, dim, cu_q != nullptr);
+  // (positions on the table and windows within 2^30 keep sums of two of them within 32 bits; a window that wide sees
+  // every key that there is)
+  if ((int64_t)width * page_size > kMaxRows)
+    return fail(XT_EUNSUPPORTED, "%s: a table of %d pages of %d tokens", what, width, page_size);
+  window = window > kMaxRows ? (int)kMaxRows : window;
+  sinks = sinks > kMaxRows ? (int)kMaxRows : sinks;
   const int64_t tiles = ((int64_t)width * page_size + kTile - 1) / kTile;    // of an entry at most
   if (tiles > 0x7FFFFFFF / x.entries || tiles * x.entries > ((int64_t)1 << 38) / kv_heads)
     return fail(XT_EUNSUPPORTED, "%s: %d row tiles over a table of %d pages", what, x.entries, width);
-  const size_t need = counter_bytes(x) + x.partials * (size_t)x.m * (dim + 4) * 4;
+  if (x.partials > kCounterSlots)
+    return fail(XT_EUNSUPPORTED, "%s: %d KV heads, at most %d", what, kv_heads, kCounterSlots / 2);
+  const size_t need = attention_bytes(x, dim);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XT_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, workspace_bytes, need);
   // no more workgroups than the table's width could keep busy
@@ -1807,7 +1815,7 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
              group, table,
              table_stride, width, seq_lens, cu_q, batch, rows, window, sinks, scale * kLog2e, out, out_row_stride,
              out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse, x.entries, kMinTiles, x.slots,
-             (int32_t*)workspace, (float*)((uint8_t*)workspace + counter_bytes(x)), x.partials};
+             (int32_t*)workspace, (float*)((uint8_t*)workspace + kCounterBytes), x.partials};
   const int m = x.m;
   if (m == 16) {
     if (dim == 64) return launch_decode<64, 1>(what, a, groups, stream);

@@ -1148,6 +1148,7 @@ def _int32(t):
     return t if t is None or (t.dtype is torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
 
 
+_MAX_WINDOW = 1 << 30     # more than any table holds
 _E4M3_BYTES = (torch.uint8, torch.float8_e4m3fn)
 
 
@@ -1159,7 +1160,7 @@ def _check_page8(what, raw):
     shape, ks, es = k.shape, k.stride(), k_exp.stride()
     if len(shape) == 4:
         pages, heads, page, dim = shape
-        if (ks[3] == 1 and ks[2] == dim and vt.shape == (pages, heads, dim, page) and k_exp.shape == shape[:2]
+        if (ks[3] == 1 and ks[2] == dim and min(ks[0], ks[1], es[0], es[1]) > 0 and vt.shape == (pages, heads, dim, page) and k_exp.shape == shape[:2]
                 and vt.stride() == (ks[0], ks[1], page, 1) and v_exp.shape == shape[:2] and v_exp.stride() == es
                 and k.dtype in _E4M3_BYTES and vt.dtype in _E4M3_BYTES and k_exp.dtype is torch.uint8
                 and v_exp.dtype is torch.uint8):
@@ -1213,13 +1214,15 @@ _stream_workspaces = {}   # (device index, stream) -> zeroed uint8 tensor
 def _stream_workspace(t, nbytes):
     """A zero-filled workspace for a call on t's device and its current stream: kept per stream, so calls that overlap
     on two streams never share one; inside a graph capture a new one of the graph's own memory, so graphs never share
-    one either."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=t.device)
+    one either. Only the arrival counters at its start have to be zero."""
+    capturing = torch._C._cuda_isCurrentStreamCapturing()
     key = (t.get_device(), _stream(t))
-    buf = _stream_workspaces.get(key)
+    buf = None if capturing else _stream_workspaces.get(key)
     if buf is None or buf.shape[0] < nbytes:
-        buf = _stream_workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=t.device)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+        buf[:_lib.COUNTER_BYTES].zero_()
+        if not capturing:
+            _stream_workspaces[key] = buf
     return buf
 
 
@@ -1258,12 +1261,12 @@ def page8_attention(q, raw, table, seq_lens, scale, cu_q=None, window=0, sinks=0
     if ws is not None and ws.dtype is not torch.uint8:
         raise ValueError('xtier_amd.page8_attention: a uint8 workspace expected')
     if ws is None:
-        ws = _stream_workspace(q, page8_workspace_bytes(rows, batch, q_heads, ptrs[5], dim) if batch else 256)
+        ws = _stream_workspace(q, page8_workspace_bytes(rows, batch, q_heads, ptrs[5], dim) or 256)
     seq_lens, cu_q = _int32(seq_lens), _int32(cu_q)
     st = _lib.lib().xt_page8_attention(
         q.data_ptr(), qs[0], qs[1], *ptrs, q_heads, dim, page, *strides, table.data_ptr(), table.stride(0),
-        table.shape[1], seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, rows, int(window),
-        int(sinks), float(scale), out.data_ptr(), os[0], os[1], out_dtype, None if lse is None else lse.data_ptr(),
+        table.shape[1], seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, rows,
+        min(int(window), _MAX_WINDOW), min(int(sinks), _MAX_WINDOW), float(scale), out.data_ptr(), os[0], os[1], out_dtype, None if lse is None else lse.data_ptr(),
         ws.data_ptr(), ws.numel(), _stream(q))
     if st:
         _lib.check(st, 'page8_attention')
@@ -1389,7 +1392,7 @@ def pages_copy(buffers, moves, count=None):
     if not isinstance(buffers, PageBuffers):
         buffers = PageBuffers(buffers)
     if moves.dim() != 2 or moves.shape[0] != 2 or moves.dtype is not torch.int32 \
-            or (moves.shape[1] > 1 and moves.stride(1) != 1) or (count is not None and count.dtype is not torch.int32):
+            or (moves.shape[1] > 1 and moves.stride(1) != 1) or (count is not None and (count.dtype is not torch.int32 or count.numel() != 1)):
         raise ValueError('xtier_amd.pages_copy: int32 moves [2, n] and an int32 count expected')
     away = _away('pages_copy', moves, count, *buffers.tensors[:1])
     if away is not None:
