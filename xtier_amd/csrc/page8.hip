@@ -1274,6 +1274,9 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
     struct Tile {
       int base;                                     // first key
       int k[ONE ? 1 : L], v;                        // pages of this thread's pieces
+      uint64_t at;                                  // ONE, once its K is loaded: the bytes to its page,
+      int ke, ve;                                   // the words that hold its exponents,
+      bool ok;                                      // and whether it has a page
     };
     Tile next;
     auto find = [&](int t) {                        // (tiles past the run repeat its last one)
@@ -1289,54 +1292,64 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
       return x;
     };
     uint4 kw[L], vw[L];
-    int kexp[ONE ? 1 : L], vexp = 0;                // exponents of the tiles to stage
+    int kexp[L], vexp = 0;                          // exponents of the tiles to stage (ONE: K's in the tile)
     bool vok = false;                               // whether the V block holds anything
     // one byte by a scalar load of the word that holds it
     auto scalar_byte = [](const uint8_t* p) {
       const uint64_t at = (uint64_t)p;
-      return uniform_load(reinterpret_cast<const int32_t*>(at & ~(uint64_t)3)) >> (8 * (int)(at & 3)) & 0xFF;
+      return uniform_load(reinterpret_cast<const int32_t*>(at & ~(uint64_t)3)) >> (8 * (int)(at & 3));
     };
-    auto load_k = [&](const Tile& x, int i) {
+    auto load_k = [&](Tile& x, int i) {
       const int32_t id = x.k[ONE ? 0 : i];
-      const uint32_t page = (uint32_t)id < a.pages ? id : 0;
       if constexpr (ONE) {
-        const uint8_t* block = k_base + (uint64_t)page * a.page_stride + (uint32_t)((x.base & page_mask) * D);
+        if (i == 0) {
+          x.ok = ((uint32_t)id < a.pages) & (x.base < en.end);
+          const uint32_t page = x.ok ? id : 0;
+          x.at = (uint64_t)page * a.page_stride;
+          const uint64_t exp = (uint64_t)page * a.exp_page_stride;
+          x.ke = scalar_byte(k_exps + exp);
+          x.ve = scalar_byte(v_exps + exp);
+        }
+        const uint8_t* block = k_base + x.at + (uint32_t)((x.base & page_mask) * D);
         kw[i] = *reinterpret_cast<const uint4*>(block + (uint32_t)(tid * 16) + 16 * T * i);
       } else {
+        const uint32_t page = (uint32_t)id < a.pages ? id : 0;
         const int piece = tid + T * i;
         kw[i] = *reinterpret_cast<const uint4*>(k_base + (uint64_t)page * a.page_stride +
                                                 (((x.base + piece / (D / 16)) & page_mask) * D + piece % (D / 16) * 16));
         kexp[i] = k_exps[(uint64_t)page * a.exp_page_stride];
       }
     };
-    // (ONE: once every piece of the tile before is converted, since they share the exponent)
-    auto load_k_exp = [&](const Tile& x) {
-      if constexpr (ONE) {
-        const uint32_t page = (uint32_t)x.k[0] < a.pages ? x.k[0] : 0;
-        kexp[0] = scalar_byte(k_exps + (uint64_t)page * a.exp_page_stride);
-      }
-    };
     const uint32_t v_off = (uint32_t)((tid >> 2) << a.page_shift) + (ONE ? 16 * (tid & 3) : 0);
     auto load_v = [&](const Tile& x, int i) {
-      const int block = ONE ? 0 : 16 * (tid & 3);
-      const bool ok = ((uint32_t)x.v < a.pages) & (x.base + block < en.end);
-      const uint32_t page = ok ? x.v : 0;
-      if (i == 0) {
-        vok = ok;
-        if constexpr (ONE) vexp = scalar_byte(v_exps + (uint64_t)page * a.exp_page_stride);
-        else vexp = v_exps[(uint64_t)page * a.exp_page_stride];
+      if constexpr (ONE) {
+        if (i == 0) {
+          vok = x.ok;
+          vexp = x.ve & 0xFF;
+        }
+        vw[i] = *reinterpret_cast<const uint4*>(v_base + x.at + (uint32_t)(x.base & page_mask) +
+                                                ((uint32_t)(16 * W * i) << a.page_shift) + v_off);
+      } else {
+        const int key = x.base + 16 * (tid & 3);
+        const bool ok = ((uint32_t)x.v < a.pages) & (key < en.end);
+        const uint32_t page = ok ? x.v : 0;
+        if (i == 0) {
+          vok = ok;
+          vexp = v_exps[(uint64_t)page * a.exp_page_stride];
+        }
+        vw[i] = *reinterpret_cast<const uint4*>(v_base + (uint64_t)page * a.page_stride + (uint32_t)(key & page_mask) +
+                                                ((uint32_t)(16 * W * i) << a.page_shift) + v_off);
       }
-      const uint8_t* vp = v_base + (uint64_t)page * a.page_stride + (uint32_t)((x.base + block) & page_mask);
-      vw[i] = *reinterpret_cast<const uint4*>(vp + ((uint32_t)(16 * W * i) << a.page_shift) + v_off);
     };
     int e_ref = 0;                                  // the exponent that O is held at once the staged tile is added
     float e_drop = 1.0f;                            // and what O is multiplied by before that
     float v_scale = 1.0f;
     uint32_t block_ok = 0;                          // bit b: the staged V tile's 16-key block b has a page
+    bool plain = false;                             // every row sees the staged tile whole
     // before V of tile t is converted into stage buf: hidden values out of the way, and its scale
     auto prepare_v = [&](int t, int buf) {
       block_ok = ONE ? (vok ? 15u : 0u) : (uint32_t)__ballot(vok) & 15u;
-      const bool plain = whole_tile(t) && t < t1 && block_ok == 15u;
+      plain = whole_tile(t) && t < t1 && block_ok == 15u;
       int ev = vexp;
       if (!plain) {
         // values of keys that no row sees may be anything, NaN included: zero them
@@ -1374,9 +1387,9 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
     // (the LDS places of a thread's first pieces; the others are a fixed number of rows further)
     const int k_put = key_row(tid / (D / 16)) * G::kRowK + tid % (D / 16) * 32;
     const int v_put = (tid >> 2) * G::kRowV + (tid & 3) * 32;
-    auto convert_k = [&](int i, int buf) {
+    auto convert_k = [&](const Tile& x, int i, int buf) {
       constexpr int kRows = T / (D / 16);           // keys between a thread's pieces: their LDS rows differ as they do
-      const float ks = exp_bits(kexp[ONE ? 0 : i]);
+      const float ks = exp_bits(ONE ? x.ke & 0xFF : kexp[i]);
       const int put = kRows % 16 == 0 ? k_put + kRows * i * G::kRowK
                                       : key_row((tid + T * i) / (D / 16)) * G::kRowK + tid % (D / 16) * 32;
       uint8_t* dst = s_k + buf * G::kStageK + put;
@@ -1411,23 +1424,21 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
     // their way together
     Tile now = find(t0);
     next = find(t0 + 1);
-    const Tile third = find(t0 + 2);
+    Tile third = find(t0 + 2);
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       load_k(now, i);
       load_v(now, i);
     }
-    load_k_exp(now);
     uint4 k_first[L];
-    int e_first[ONE ? 1 : L];
+    int e_first[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       k_first[i] = kw[i];
-      e_first[ONE ? 0 : i] = kexp[ONE ? 0 : i];
+      e_first[i] = kexp[i];
     }
 #pragma unroll
     for (int i = 0; i < L; ++i) load_k(next, i);
-    load_k_exp(next);
     prepare_v(t0, 0);
 #pragma unroll
     for (int i = 0; i < L; ++i) convert_v(i, 0);
@@ -1435,19 +1446,19 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
     for (int i = 0; i < L; ++i) load_v(next, i);
     float drop = e_drop;                // of the tile whose PV comes next
     uint32_t tile_ok = block_ok;
+    bool tile_plain = plain;
 #pragma unroll
-    for (int i = 0; i < L; ++i) convert_k(i, 1);
+    for (int i = 0; i < L; ++i) convert_k(next, i, 1);
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       kw[i] = k_first[i];
-      kexp[ONE ? 0 : i] = e_first[ONE ? 0 : i];
+      kexp[i] = e_first[i];
     }
 #pragma unroll
-    for (int i = 0; i < L; ++i) convert_k(i, 0);
+    for (int i = 0; i < L; ++i) convert_k(now, i, 0);
     now = third;
 #pragma unroll
     for (int i = 0; i < L; ++i) load_k(now, i);
-    load_k_exp(now);
     next = find(t0 + 3);                // in the step of t: `now` is tile t + 2, its K loaded; `next` t + 3
     __syncthreads();
     float16_t s0[2], s1[2];
@@ -1466,7 +1477,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
       constexpr int B = decltype(stage)::value;
       // s[kb][4 a + i] is key base + 32 kb + 16 (a / 2) + 8 hf + 4 (a % 2) + i
       uint32_t vis = 0xFFFFFFFFu;
-      if (!whole_tile(t) || tile_ok != 15u) {
+      const bool hidden = !tile_plain;
+      if (hidden) {
         vis = 0;                              // bit 16 kb + i
         const Sight sight = sight_of(a, pos, pos, en.end, key_of(t) + 8 * hf);
 #pragma unroll
@@ -1526,7 +1538,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
         __builtin_amdgcn_sched_barrier(0);
       }
       l_run = l_run * alpha + sum;
-      if (!whole_tile(t) && s_nan[t & 3]) {
+      if (hidden && s_nan[t & 3]) {
         // vis holds keys 16 u + 8 hf + i as bit 8 u + i: the row's 16-bit blocks are its bytes and the other half's
         const auto sw = __builtin_amdgcn_permlane32_swap(vis, vis, false, false);
         const uint32_t low = sw[0], high = sw[1];
@@ -1548,6 +1560,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
       prepare_v(t + 1, B ^ 1);
       drop = e_drop;
       tile_ok = block_ok;
+      tile_plain = plain;
       // this tile's values beside the conversion of the next V and the K after it, each register refilled once it is
       // converted
       half8_t vf[2][G::kDT];
@@ -1570,13 +1583,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
             load_v(now, i);
           }
           if ((2 * i + 1) * 4 / (2 * L) == u) {
-            convert_k(i, B);
+            convert_k(now, i, B);
             load_k(next, i);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      load_k_exp(next);
       now = next;
       next = find(t + 4);
       if (tid == 0) s_nan[(t + 2) & 3] = 0;      // read last two steps ago
