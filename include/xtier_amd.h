@@ -366,7 +366,8 @@ int xt_sparse_mla_fp8(const void* q, int64_t q_row_stride, int64_t q_head_stride
  *
  * Requests: seq_lens[b] is request b's length with its new tokens; its rows of k / v or q are cu[b] .. cu[b + 1] - 1
  * (int32 [batch + 1], not decreasing, cu[batch] <= rows; NULL: one row each, rows == batch), at the positions
- * seq_lens[b] - n .. seq_lens[b] - 1 for n rows. A negative length counts as 0. */
+ * seq_lens[b] - n .. seq_lens[b] - 1 for n rows. A negative length counts as 0. Pages (and their
+ * scales) less than 2^32 bytes apart. */
 
 /* Quantize-on-append of K and V rows (BF16 [rows, kv_heads, dim], strides in elements, 16-byte aligned rows). For every
  * page and head that takes rows, K and V alike:
@@ -393,15 +394,16 @@ size_t xt_page8_attention_workspace_bytes(int rows, int batch, int q_heads, int 
  * visible), as far as pages hold them:
  *   out[r, h] = sum_j softmax_j(q[r, h] . k_j * scale) v_j,   lse[r, h] = ln sum_j exp(q[r, h] . k_j * scale).
  * Pages that no row sees (behind the window) may be freed: their table entries are not followed, or only to masked
- * keys. Whatever hidden places hold, NaN included, changes nothing. A row that sees no key gives 0 and -inf; rows of q
- * behind cu_q[batch] are left as they are. q: BF16 [rows, q_heads, dim] (strides in elements, 16-byte aligned rows);
- * q_heads / kv_heads <= 128; scale > 0; out: out_dtype (strides in elements, 8-byte aligned rows); lse (optional): FP32
+ * keys. Whatever hidden places hold, NaN included, changes nothing. A row that sees no key (or only scores of -inf, which
+ * an infinite query makes) gives 0 and -inf; rows of q behind cu_q[batch] are left as they are. q: BF16 [rows, q_heads,
+ * dim] (strides in elements, 16-byte aligned rows); q_heads / kv_heads <= 128; scale > 0; out: out_dtype (strides in elements, 8-byte aligned rows); lse (optional): FP32
  * [rows, q_heads]. QK exact products of BF16 with FP32 sums; P and V as FP16 in the second product (V exact within 15
  * binades of scale below the largest of the row's pages), FP32 sums.
  * workspace: xt_page8_attention_workspace_bytes bytes, 256-byte aligned. It begins with the 64 KB of arrival counters that
  * the other decode entry points have too, zero before the first use and left zero; calls of any shape may share one, one
- * at a time. Tables of up to 2^30 tokens and kv_heads <= 8192. One launch on `stream`, its work divided on the device,
- * so that a captured launch follows the lengths of each replay. */
+ * at a time. Tables of up to 2^30 tokens, kv_heads <= 8192, and row tiles (of 16 rows x heads of a group and more) times
+ * kv_heads below 2^23. One launch on `stream`, or for large batches (over 64 row tiles, 256 or more for prompts) two; the
+ * work is divided on the device, so that a captured call follows the lengths of each replay. */
 int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const uint8_t* k_pages,
                        const uint8_t* vt_pages, const uint8_t* k_exp, const uint8_t* v_exp, int64_t pages, int kv_heads,
                        int q_heads, int dim, int page_size, int64_t page_stride, int64_t head_stride,
@@ -423,7 +425,7 @@ int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
 size_t xt_pages_workspace_bytes(int64_t pages);
 
 /* Each row b grows by add[b] >= 0 tokens: it gets the pages that ceil((lens[b] + add[b]) / page_size) columns need, and
- * lens[b] += add[b]. Rows are served in order: a row whose pages, with those that the rows before it asked for, are more
+ * lens[b] += add[b] (width < 2^21). Rows are served in order: a row whose pages, with those that the rows before it asked for, are more
  * than the free ones gets none and keeps its length, and so does a row that would outgrow the table; granted[b]
  * (uint8) says which grew. */
 int xt_pages_extend(int32_t* refs, int64_t pages, int32_t* table, int64_t table_stride, int width, int32_t* lens,

@@ -70,6 +70,10 @@ def attention_on_gpu(q, raw, table, page, lens, scale, cu, window=0, sinks=0):
     lse, score = (torch.empty(q.shape[:2], dtype=torch.float64, device='cuda') for _ in range(2))
     for b, length in enumerate(lens.tolist()):
         lo, hi = int(cu[b]), int(cu[b + 1])
+        if length <= 0:
+            out[lo:hi] = spread[lo:hi] = score[lo:hi] = 0
+            lse[lo:hi] = -np.inf
+            continue
         ids = torch.from_numpy(table[b, :-(-length // page)].astype(np.int64)).cuda()
         p = torch.arange(length - (hi - lo), length, device='cuda')
         for h in range(k8.shape[1]):
@@ -84,7 +88,7 @@ def attention_on_gpu(q, raw, table, page, lens, scale, cu, window=0, sinks=0):
                 qq = q[lo:hi, g]
                 z = (qq @ k.t() * scale).masked_fill(~seen, -np.inf)
                 lse[lo:hi, g] = torch.logsumexp(z, 1)
-                w = torch.exp(z - lse[lo:hi, g, None])
+                w = torch.exp(z - lse[lo:hi, g, None]).masked_fill(~seen, 0)       # (a row may see nothing)
                 out[lo:hi, g], spread[lo:hi, g] = w @ v, w @ v.abs()
                 score[lo:hi, g] = (qq.abs() @ k.abs().t()).masked_fill(~seen, 0).amax(1) * scale
     return tuple(x.cpu().numpy() for x in (out, lse, spread, score))

@@ -333,6 +333,44 @@ def test_many_requests():
     _check_attention(*_attention_case(rng, lens, [40] * 130, 16, 1, 4, 64), 16, large=True)
 
 
+@pytest.mark.parametrize('dim,heads,group,n,most,window', [
+    (128, 1, 2, 2500, 1, 0),        # decode: several entries to a thread of the plan
+    (64, 2, 4, 70, 8, 0), (128, 2, 8, 90, 4, 100), (256, 1, 8, 70, 4, 0),        # 32 rows each
+    (64, 1, 16, 70, 4, 50),         # 64 rows each
+    (128, 2, 2, 540, 60, 0), (256, 1, 3, 300, 60, 90), (64, 3, 3, 300, 60, 0)])   # prompts
+def test_large_batches(dim, heads, group, n, most, window):
+    """More row tiles than a workgroup divides by itself: requests of 0 to `most` rows, one of them far longer than the
+    others, one without tokens."""
+    rng = np.random.default_rng(dim + n)
+    rows = rng.integers(most // 2, most + 1, n) if most > 1 else rng.integers(0, 2, n)
+    lens = np.maximum(rows, 1) + rng.integers(0, 40, n)
+    lens[n // 3], rows[n // 2], lens[n // 5] = 5000, most, rows[n // 5]
+    raw, table, lens, cu, q = _attention_case(rng, lens.tolist(), rows.tolist(), 16, heads, group, dim)
+    _check_attention(raw, table, lens, cu, q, 16, window, 3 if window else 0, large=True)
+
+
+def test_a_large_batch_in_a_graph():
+    """A replay follows lengths that changed, where a plan is made on the device too."""
+    rng = np.random.default_rng(36)
+    n = 200
+    raw, table, lens, cu, q = _attention_case(rng, rng.integers(200, 900, n).tolist(), [1] * n, 32, 2, 4, 64)
+    pool, q, table, lens = gpu_raw(raw), q.cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda()
+    out = torch.empty_like(q)
+    pool.attend(q, table, lens, 0.02)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pool.attend(q, table, lens, 0.02, out=out)
+    for step in range(4):
+        lens.sub_(step * 60).clamp_(min=1)
+        lens[17 * step] = table.shape[1] * 32 if step == 2 else 5
+        want = pool.attend(q, table, lens, 0.02)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_calls_of_differing_shapes_share_a_workspace():
     """Calls whose partials lie at different places, one after the other in one workspace: each finds its counters zero."""
     rng = np.random.default_rng(34)

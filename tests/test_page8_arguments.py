@@ -66,6 +66,19 @@ def test_attention(lib):
     assert lib.xt_page8_attention_workspace_bytes(1, 2, 30, 4, 128) == 0
 
 
+def test_calls_too_large_for_one_launch(lib):
+    assert _append(lib, rows=1 << 30, cu=P) == _lib.XT_EUNSUPPORTED
+    assert _append(lib, rows=1 << 27, cu=None, batch=1 << 27) == _lib.XT_EUNSUPPORTED
+    assert _attend(lib, rows=1 << 21, batch=1 << 21) == _lib.XT_EUNSUPPORTED
+    assert b'row tiles of 4 KV heads' in lib.xt_last_error()
+    assert lib.xt_pages_free(P, 100, P, 9, 9, P, 3, P, 1 << 24, None) == _lib.XT_EUNSUPPORTED
+    # a large batch's workspace holds its plan too
+    one, many = (lib.xt_page8_attention_workspace_bytes(n, n, 32, 4, 128) for n in (40, 4000))
+    assert many > one + 4000 * 32
+    assert _attend(lib, rows=4000, batch=4000, ws_bytes=many - 1) in (_lib.XT_EWORKSPACE, _lib.XT_ELAUNCH)
+    assert _attend(lib, rows=4000, batch=4000, ws_bytes=one) == _lib.XT_EWORKSPACE
+
+
 def test_page_operators(lib):
     ok, bad, small, far = _lib.XT_OK, _lib.XT_EINVAL, _lib.XT_EWORKSPACE, _lib.XT_EUNSUPPORTED
     assert lib.xt_pages_workspace_bytes(100) == 400 and lib.xt_pages_workspace_bytes(-1) == 0

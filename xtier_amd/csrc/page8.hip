@@ -210,6 +210,12 @@ __global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
 
 // --- attention: the work and its division ------------------------------------------------------------------------------
 
+// A piece of a planned call: its request and row tile, and which of its entry's pieces it is; with more than one, the
+// slot of its partial within the head.
+struct Planned {
+  int b, tile, at, count, slot, pad[3];
+};
+
 struct AttnArgs {
   const uint16_t* q;
   int64_t q_row, q_head;
@@ -235,6 +241,9 @@ struct AttnArgs {
   int32_t* counters;    // one per partial, zero between calls
   float* part;
   int partials;         // what `part` has room for
+  int* plan;            // of a call with many entries, else NULL: pieces of a head, those of cut entries among them
+  Planned* planned;     // and its pieces
+  int* plan_tiles;      // scratch, an entry each
 };
 
 // A row tile of a request: rows r = token * group + head of the group, `m_rows` of them, and its key tiles. Tile t of
@@ -251,27 +260,33 @@ struct Entry {
 // The row tiles of the requests before one whose first row is `row`, some of them empty.
 __device__ inline int tile_base(const AttnArgs& a, int row, int m_rows) { return row * a.group / m_rows; }
 
-__device__ inline Entry entry_at(const AttnArgs& a, int e, int m_rows) {
-  Entry x;
-  int tile;
+// The request and row tile of an entry.
+__device__ inline int request_of(const AttnArgs& a, int e, int m_rows, int* tile) {
   if (!a.cu_q) {
-    const int per = (a.group + m_rows - 1) / m_rows;
-    x.b = per == 1 ? e : e / per;
-    tile = e - x.b * per;
-    x.row0 = x.b;
+    const int per = (a.group + m_rows - 1) / m_rows, b = per == 1 ? e : e / per;
+    *tile = e - b * per;
+    return b;
+  }
+  // request b's tiles start at floor(cu[b] * group / m_rows) + b, which leaves room for a ragged last one
+  int lo = 0, hi = a.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tile_base(a, a.cu_q[mid], m_rows) + mid <= e) lo = mid;
+    else hi = mid - 1;
+  }
+  *tile = e - (tile_base(a, a.cu_q[lo], m_rows) + lo);
+  return lo;
+}
+
+__device__ inline Entry entry_of(const AttnArgs& a, int b, int tile, int m_rows) {
+  Entry x;
+  x.b = b;
+  if (!a.cu_q) {
+    x.row0 = b;
     x.n = 1;
   } else {
-    // request b's tiles start at floor(cu[b] * group / m_rows) + b, which leaves room for a ragged last one
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (tile_base(a, a.cu_q[mid], m_rows) + mid <= e) lo = mid;
-      else hi = mid - 1;
-    }
-    x.b = lo;
-    x.row0 = a.cu_q[lo];
-    x.n = a.cu_q[lo + 1] - x.row0;
-    tile = e - (tile_base(a, x.row0, m_rows) + lo);
+    x.row0 = a.cu_q[b];
+    x.n = a.cu_q[b + 1] - x.row0;
     if (x.row0 < 0 || x.n < 0 || x.row0 + (int64_t)x.n > a.rows) x.n = 0;
   }
   x.len = max(a.seq_lens[x.b], 0);
@@ -298,9 +313,18 @@ __device__ inline Entry entry_at(const AttnArgs& a, int e, int m_rows) {
   return x;
 }
 
+__device__ inline Entry entry_at(const AttnArgs& a, int e, int m_rows) {
+  int tile;
+  const int b = request_of(a, e, m_rows, &tile);
+  return entry_of(a, b, tile, m_rows);
+}
+
 // Both kernels divide their work, the key tiles of every (KV head, entry), on the device: a long request is shared by
 // many workgroups, whatever the lengths, and a captured launch follows the lengths of each replay. Work is numbered head
-// by head, entry by entry. A (head, entry) that several workgroups share is merged from their partials by the last of
+// by head, entry by entry. Every workgroup divides the work for itself if there is at most one entry to a lane (decode) or
+// thread (prefill); of more, a launch before makes the plan (plan_kernel): in every workgroup again, the division grew
+// with the square of the entries (decode of 1024 requests of 256 keys, with row offsets: 459 us, now 77; of 8192: 40 ms,
+// now 565 us; of 256: 53, now 27). A (head, entry) that several workgroups share is merged from their partials by the last of
 // them to finish, in their order.
 //
 // Sums of x and y over the workgroup's threads before this one, and over all of them. `s` holds 2 * T / 64 values.
@@ -334,9 +358,9 @@ __device__ inline void block_sums(int x, int y, int* s, int* x_before, int* x_al
 // as small as leaves all of them on the CUs at once (or, with more (head, entry) pairs than half the slots, only those
 // well above the mean are cut: a piece has at most total / (slots / 2) tiles). Cutting at pairs only keeps every
 // workgroup at one entry: equal runs that cross from one to the next cost a second entry's loads and merges in a row,
-// 8 us (measured: 1 request, 2 KV heads x 256, 4099 keys, 25 us).
+// 8 us (1 request, 2 KV heads x 256, 4099 keys: 25 us so, 17 now).
 struct Piece {
-  int head, entry, at, count;
+  int head, at, count;
   int slot;              // of the piece's partial, if count > 1; the slots of an entry's pieces are neighbours
 };
 
@@ -358,89 +382,137 @@ __device__ inline int piece_of_xcd(int id, int count) {
   return (id >> 3) < of_xcd && w < count ? w : -1;
 }
 
-template <int T>
-__device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id) {
+// Where the pieces of a head under the least size are more than there is room for: how many a second size is meant to give,
+// besides one for each entry.
+__device__ inline int sure_pieces(int room, int n_live) { return max(max(room - n_live, room / 2), 1); }
+
+__device__ inline Piece planned_piece(const AttnArgs& a, int id, int m_rows, Entry* en) {
+  Piece x;
+  x.count = 0;
+  const int per_head = uniform_load(a.plan);
+  const int w = piece_of_xcd(id, per_head * a.heads);
+  if (w < 0) return x;
+  x.head = w / per_head;
+  const int* p = &a.planned[w - x.head * per_head].b;
+  *en = entry_of(a, uniform_load(p), uniform_load(p + 1), m_rows);
+  x.at = uniform_load(p + 2);
+  x.count = uniform_load(p + 3);
+  x.slot = x.head * uniform_load(a.plan + 1) + uniform_load(p + 4);
+  return x;
+}
+
+// An entry to a lane, every wave by itself: no barriers (1 request of 4099 keys, 18.5 us with them, 17.3 without).
+__device__ inline Piece piece_of(const AttnArgs& a, int m_rows, int id, Entry* en) {
   Piece x;
   x.count = 0;
   const int room = max(a.slots / a.heads, 1);       // pieces of a head
-  if (a.entries <= 64) {
-    // an entry to a lane, every wave by itself: no barriers (1 request of 4099 keys, 18.5 us with them, 17.3 without)
-    const int lane = (int)threadIdx.x & 63;
-    const int tiles = lane < a.entries ? entry_at(a, lane, m_rows).tiles : 0;
-    const int all = __builtin_amdgcn_readlane(wave_inclusive_sum(tiles), 63);
-    const int n_live = __popcll(__ballot(tiles > 0)), sure = max(max(room - n_live, room / 2), 1);
-    const int least = least_piece(a, m_rows, all, n_live);
-    int size = max((all + room - 1) / room, least), n, upto, cut;
-    for (int tries = 0;; ++tries) {
-      n = (tiles + size - 1) / size;
-      upto = wave_inclusive_sum(n);
-      cut = wave_inclusive_sum(n > 1 ? n : 0);
-      if (__builtin_amdgcn_readlane(upto, 63) <= room || tries == 1) break;
-      size = max((all + sure - 1) / sure, least);
-    }
-    const int per_head = __builtin_amdgcn_readlane(upto, 63), cut_per_head = __builtin_amdgcn_readlane(cut, 63);
-    const int w = piece_of_xcd(id, per_head * a.heads);
-    if (w < 0) return x;
-    x.head = w / per_head;
-    const int want = w - x.head * per_head;
-    x.entry = __builtin_ctzll(__ballot(want < upto));          // the first entry whose running count passes it
-    x.count = __builtin_amdgcn_readlane(n, x.entry);
-    x.at = want - (__builtin_amdgcn_readlane(upto, x.entry) - x.count);
-    x.slot = x.head * cut_per_head + __builtin_amdgcn_readlane(cut, x.entry) - x.count + x.at;
-    return x;
+  const int lane = (int)threadIdx.x & 63;
+  const Entry mine = entry_at(a, min(lane, a.entries - 1), m_rows);
+  const int tiles = lane < a.entries ? mine.tiles : 0;
+  const int all = __builtin_amdgcn_readlane(wave_inclusive_sum(tiles), 63);
+  const int n_live = __popcll(__ballot(tiles > 0)), sure = sure_pieces(room, n_live);
+  const int least = least_piece(a, m_rows, all, n_live);
+  // per head: the smallest size that could fit, and if it does not, one that is sure to
+  int size = max((all + room - 1) / room, least), n, upto, cut;
+  for (int tries = 0;; ++tries) {
+    n = (tiles + size - 1) / size;
+    upto = wave_inclusive_sum(n);
+    cut = wave_inclusive_sum(n > 1 ? n : 0);
+    if (__builtin_amdgcn_readlane(upto, 63) <= room || tries == 1) break;
+    size = max((all + sure - 1) / sure, least);
   }
+  const int per_head = __builtin_amdgcn_readlane(upto, 63), cut_per_head = __builtin_amdgcn_readlane(cut, 63);
+  const int w = piece_of_xcd(id, per_head * a.heads);
+  if (w < 0) return x;
+  x.head = w / per_head;
+  const int want = w - x.head * per_head;
+  const int entry = __builtin_ctzll(__ballot(want < upto));    // the first entry whose running count passes it
+  x.count = __builtin_amdgcn_readlane(n, entry);
+  x.at = want - (__builtin_amdgcn_readlane(upto, entry) - x.count);
+  x.slot = x.head * cut_per_head + __builtin_amdgcn_readlane(cut, entry) - x.count + x.at;
+  // (from its lane: loading it again would cost another round trip)
+  auto of_entry = [&](int v) { return __builtin_amdgcn_readlane(v, entry); };
+  en->b = of_entry(mine.b);
+  en->n = of_entry(mine.n);
+  en->row0 = of_entry(mine.row0);
+  en->r0 = of_entry(mine.r0);
+  en->r1 = of_entry(mine.r1);
+  en->len = of_entry(mine.len);
+  en->start = of_entry(mine.start);
+  en->end = of_entry(mine.end);
+  en->sink_tiles = of_entry(mine.sink_tiles);
+  en->skip = of_entry(mine.skip);
+  en->tiles = of_entry(mine.tiles);
+  return x;
+}
+
+// The plan of a call with many entries, by one workgroup: a run of entries to a thread. `room`: pieces of a head at once.
+// Decode (`few` rows) cuts as piece_of does. Prefill, whose workgroups take pieces in rounds, cuts only entries that are
+// longer than an equal share of all of them. Either way an entry that is cut is longer than a size that goes at most
+// `room` times into their sum, so that the pieces with partials are fewer than 2 * room.
+constexpr int kPlanThreads = 1024;
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttnArgs a, int m_rows, int room, bool few) {
+  constexpr int T = kPlanThreads;
   __shared__ int s_sum[2 * (T / 64)];
-  __shared__ int s_find[4];
   const int tid = (int)threadIdx.x;
   const int chunk = (a.entries + T - 1) / T;
-  const int e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
-  int sum = 0, live = 0, tiles = 0, before, all, cut_before, n_live;
-  for (int e = e0; e < e1; ++e) {
-    tiles = entry_at(a, e, m_rows).tiles;
-    sum += tiles;
-    live += tiles > 0;
-  }
-  auto tiles_of = [&](int e) { return chunk == 1 ? tiles : entry_at(a, e, m_rows).tiles; };
+  const int e0 = (int)min((int64_t)chunk * tid, (int64_t)a.entries), e1 = min(e0 + chunk, a.entries);
+  int first_tile = 0;
+  const int first = e0 < e1 ? request_of(a, e0, m_rows, &first_tile) : 0;
+  // the entries of this thread in order: f(entry, request, row tile); with offsets, the requests are walked through
+  auto each = [&](auto f) {
+    int b = first, tile = first_tile;
+    const int per = (a.group + m_rows - 1) / m_rows;
+    for (int e = e0; e < e1; ++e) {
+      f(e, b, tile);
+      ++tile;
+      if (!a.cu_q) {
+        if (tile == per) {
+          ++b;
+          tile = 0;
+        }
+      } else {
+        int base;
+        while (b + 1 < a.batch && (base = tile_base(a, a.cu_q[b + 1], m_rows) + b + 1) <= e + 1) {
+          ++b;
+          tile = e + 1 - base;
+        }
+      }
+    }
+  };
+  int sum = 0, live = 0, before, all, cut_before, n_live;
+  each([&](int e, int b, int tile) {
+    const int t = entry_of(a, b, tile, m_rows).tiles;
+    a.plan_tiles[e] = t;
+    sum += t;
+    live += t > 0;
+  });
   block_sums<T>(sum, live, s_sum, &before, &all, &cut_before, &n_live);
-  // per head: the smallest size that could fit, and if it does not, one that is sure to
-  const int sure = max(max(room - n_live, room / 2), 1), least = least_piece(a, m_rows, all, n_live);
+  const int sure = few ? sure_pieces(room, n_live) : room;
+  const int least = few ? least_piece(a, m_rows, all, n_live) : a.min_tiles;
   int size = max((all + room - 1) / room, least), mine, cut, per_head, cut_per_head;
   for (int tries = 0;; ++tries) {
     mine = cut = 0;
     for (int e = e0; e < e1; ++e) {
-      const int n = (tiles_of(e) + size - 1) / size;
+      const int n = (a.plan_tiles[e] + size - 1) / size;
       mine += n;
       cut += n > 1 ? n : 0;
     }
     block_sums<T>(mine, cut, s_sum, &before, &per_head, &cut_before, &cut_per_head);
-    if (per_head <= room || tries == 1) break;
+    if (!few || per_head <= room || tries == 1) break;
     size = max((all + sure - 1) / sure, least);
   }
-  const int w = piece_of_xcd(id, per_head * a.heads);
-  if (w < 0) return x;
-  x.head = w / per_head;
-  int want = w - x.head * per_head - before;        // the piece, counted from this thread's first
-  if (want >= 0 && want < mine) {
-    for (int e = e0; e < e1; ++e) {
-      const int n = (tiles_of(e) + size - 1) / size;
-      if (want < n) {
-        s_find[0] = e;
-        s_find[1] = want;
-        s_find[2] = n;
-        s_find[3] = cut_before + want;
-        break;
-      }
-      want -= n;
-      cut_before += n > 1 ? n : 0;
-    }
+  if (tid == 0) {
+    a.plan[0] = per_head;
+    a.plan[1] = cut_per_head;
   }
-  __syncthreads();
-  x.entry = __builtin_amdgcn_readfirstlane(s_find[0]);
-  x.at = __builtin_amdgcn_readfirstlane(s_find[1]);
-  x.count = __builtin_amdgcn_readfirstlane(s_find[2]);
-  x.head = __builtin_amdgcn_readfirstlane(x.head);
-  x.slot = x.head * cut_per_head + __builtin_amdgcn_readfirstlane(s_find[3]);
-  return x;
+  int at = before, slot = cut_before;
+  each([&](int e, int b, int tile) {
+    const int n = (a.plan_tiles[e] + size - 1) / size;
+    for (int i = 0; i < n; ++i) a.planned[at + i] = Planned{b, tile, i, n, slot + i, {0, 0, 0}};
+    at += n;
+    slot += n > 1 ? n : 0;
+  });
 }
 
 // The workgroup of the launch, renumbered so that each XCD (workgroups go round robin over 8) takes a contiguous run of
@@ -480,18 +552,21 @@ __device__ inline Run plan_run(const AttnArgs& a, int m_rows, int groups, int id
                                 Segment* sg) {
   Run x;
   const int tid = (int)threadIdx.x;
-  const int chunk = (a.entries + T - 1) / T;
-  const int e0 = min(chunk * tid, a.entries), e1 = min(e0 + chunk, a.entries);
-  int sum = 0, live = 0, most = 0, before, all, cut_before, n_live;
-  for (int e = e0; e < e1; ++e) {
-    const int t = entry_at(a, e, m_rows).tiles;
-    sum += t;
-    live += t > 0;
-    most = max(most, t);
+  x.turn = 0;
+  x.pos = x.end = 0;
+  sg->head = sg->entry = sg->t0 = sg->t1 = 0;
+  if (a.plan) {
+    x.pieces = true;
+    x.per_head = uniform_load(a.plan);
+    x.cut_per_head = uniform_load(a.plan + 1);
+    return x;
   }
+  const int tiles = tid < a.entries ? entry_at(a, tid, m_rows).tiles : 0;
+  int before, all, cut_before, n_live;
   if (tid == 0) s_find[0] = 0;
-  block_sums<T>(sum, live, s_sum, &before, &all, &cut_before, &n_live);
-  atomicMax(&s_find[0], most);
+  block_sums<T>(tiles, tiles > 0, s_sum, &before, &all, &cut_before, &n_live);
+  atomicMax(&s_find[0], tiles);
+  int most;
   __syncthreads();
   most = __builtin_amdgcn_readfirstlane(s_find[0]);
   all = __builtin_amdgcn_readfirstlane(all);
@@ -516,26 +591,18 @@ __device__ inline Run plan_run(const AttnArgs& a, int m_rows, int groups, int id
     }
   }
   x.pieces = by_pieces <= by_runs;
-  x.turn = 0;
   x.per = max(run, a.min_tiles);
-  x.pos = x.end = 0;
   x.per_head = all;
-  sg->head = sg->entry = sg->t0 = sg->t1 = 0;
   if (x.pieces) {
-    // s_mine: of each thread's entries, the pieces before them, theirs, and the cut ones before them (in LDS: in
-    // registers they would stay through the whole kernel)
-    int mine, cut;
+    // s_mine: the pieces before each thread's entry, its own, and the cut ones before it (in LDS: in registers they would
+    // stay through the whole kernel)
+    int mine;
     const int room = max(groups / a.heads, 1), tight = max((all + room - 1) / room, a.min_tiles);
     const bool try_tight = size < most && tight < size;      // the smallest size that could fit, else the sure one
     for (int tries = try_tight ? 0 : 1;; ++tries) {
       x.size = max(tries == 0 ? tight : size, 1);
-      mine = cut = 0;
-      for (int e = e0; e < e1; ++e) {
-        const int n = (entry_at(a, e, m_rows).tiles + x.size - 1) / x.size;
-        mine += n;
-        cut += n > 1 ? n : 0;
-      }
-      block_sums<T>(mine, cut, s_sum, &before, &x.per_head, &cut_before, &x.cut_per_head);
+      mine = (tiles + x.size - 1) / x.size;
+      block_sums<T>(mine, mine > 1 ? mine : 0, s_sum, &before, &x.per_head, &cut_before, &x.cut_per_head);
       if (tries == 1 || __builtin_amdgcn_readfirstlane(x.per_head) <= room) break;
     }
     x.size = __builtin_amdgcn_readfirstlane(x.size);
@@ -553,17 +620,9 @@ __device__ inline Run plan_run(const AttnArgs& a, int m_rows, int groups, int id
   sg->head = (int)(x.pos / all);
   const int want = (int)(x.pos - (int64_t)sg->head * all);   // within the head
   __syncthreads();
-  if (want >= before && want < before + sum) {
-    int at = before;
-    for (int e = e0; e < e1; ++e) {
-      const int t = entry_at(a, e, m_rows).tiles;
-      if (want < at + t) {
-        s_find[0] = e;
-        s_find[1] = at;
-        break;
-      }
-      at += t;
-    }
+  if (want >= before && want < before + tiles) {
+    s_find[0] = tid;
+    s_find[1] = before;
   }
   __syncthreads();
   sg->entry = __builtin_amdgcn_readfirstlane(s_find[0]);
@@ -580,33 +639,32 @@ __device__ inline bool next_segment(const AttnArgs& a, int m_rows, int groups, i
     ++x.turn;
     if (w < 0) return false;
     sg->head = w / x.per_head;
-    const int tid = (int)threadIdx.x;
-    int want = w - sg->head * x.per_head - s_mine[tid], rank = s_mine[2 * T + tid];
-    __syncthreads();
-    if (want >= 0 && want < s_mine[T + tid]) {
-      const int chunk = (a.entries + T - 1) / T, e0 = chunk * tid;
-      for (int e = e0; e < min(e0 + chunk, a.entries); ++e) {
-        const int n = (entry_at(a, e, m_rows).tiles + x.size - 1) / x.size;
-        if (want < n) {
-          s_find[0] = e;
-          s_find[1] = want;
-          s_find[2] = n;
-          s_find[3] = rank;
-          break;
-        }
-        want -= n;
-        rank += n > 1 ? n : 0;
+    int slot;                            // of the entry's first piece, among those of its head
+    if (a.plan) {
+      const int* p = &a.planned[w - sg->head * x.per_head].b;
+      *en = entry_of(a, uniform_load(p), uniform_load(p + 1), m_rows);
+      sg->at = uniform_load(p + 2);
+      sg->sharers = uniform_load(p + 3);
+      slot = uniform_load(p + 4) - sg->at;
+    } else {
+      const int tid = (int)threadIdx.x, want = w - sg->head * x.per_head - s_mine[tid];
+      __syncthreads();
+      if (want >= 0 && want < s_mine[T + tid]) {
+        s_find[0] = tid;
+        s_find[1] = want;
+        s_find[2] = s_mine[T + tid];
+        s_find[3] = s_mine[2 * T + tid];
       }
+      __syncthreads();
+      *en = entry_at(a, __builtin_amdgcn_readfirstlane(s_find[0]), m_rows);
+      sg->at = __builtin_amdgcn_readfirstlane(s_find[1]);
+      sg->sharers = __builtin_amdgcn_readfirstlane(s_find[2]);
+      slot = __builtin_amdgcn_readfirstlane(s_find[3]);
     }
-    __syncthreads();
-    sg->entry = __builtin_amdgcn_readfirstlane(s_find[0]);
-    sg->at = __builtin_amdgcn_readfirstlane(s_find[1]);
-    sg->sharers = __builtin_amdgcn_readfirstlane(s_find[2]);
-    *en = entry_at(a, sg->entry, m_rows);
     const int share = en->tiles / sg->sharers, longer = en->tiles % sg->sharers;   // the first `longer` have one more
     sg->t0 = sg->at * share + min(sg->at, longer);
     sg->t1 = sg->t0 + share + (sg->at < longer ? 1 : 0);
-    sg->base = sg->counter = sg->head * x.cut_per_head + __builtin_amdgcn_readfirstlane(s_find[3]);
+    sg->base = sg->counter = sg->head * x.cut_per_head + slot;
     sg->step = 1;
     sg->bump = 0;
     return true;
@@ -851,11 +909,11 @@ __global__ __launch_bounds__(256, decode_per_cu(D)) void decode_kernel(AttnArgs 
   __shared__ int s_last;
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const Piece pc = piece_of<256>(a, M, (int)blockIdx.x);
+  Entry en;
+  const Piece pc = a.plan ? planned_piece(a, (int)blockIdx.x, M, &en) : piece_of(a, M, (int)blockIdx.x, &en);
   if (pc.count == 0) return;
   const int page_mask = (1 << a.page_shift) - 1;
   const int kk0 = 16 * (c >> 2) + (c & 3);   // A row c of 16-key tile t is key kk0 + 4 t of the 64
-  const Entry en = entry_at(a, pc.entry, M);
   const int head = pc.head;
   const int share = en.tiles / pc.count, longer = en.tiles % pc.count;    // the first `longer` pieces have a tile more
   const int t0 = pc.at * share + min(pc.at, longer), t1 = t0 + share + (pc.at < longer ? 1 : 0);
@@ -1662,11 +1720,13 @@ int tile_rows(int64_t rows, int batch, int group, int dim) {
 }
 
 constexpr int64_t kMaxRows = 1 << 30;   // rows x heads of a group: 32-bit row numbers in the kernels
+constexpr int64_t kMaxUnits = 1 << 23;  // (KV head, row tile) pairs: the threads of a launch stay below 2^32
 constexpr int kMinTiles = 4;   // key tiles of a workgroup at least: one for each wave of the decode kernel
 
 struct Launch {
   int m, entries, slots, groups;
   int partials;                // of m rows each
+  int planned;                 // pieces of a head that a plan has room for, 0 without one
 };
 
 // The prefill kernel has one workgroup to a slot, each with at
@@ -1681,14 +1741,19 @@ Launch plan_launch(int rows, int batch, int heads, int group, int dim, bool ragg
   const int per_cu = prefill ? (x.m == 256 || dim == 256 ? 1 : 2) : decode_per_cu(dim);
   x.slots = per_cu * device_cus() / 8 * 8;
   const int64_t units = (int64_t)x.entries * heads, room = x.slots > heads ? x.slots : heads;
-  x.groups = prefill ? x.slots : (int)((units + room + 7) / 8 * 8);
+  x.groups = prefill ? x.slots : (int)((units < kMaxUnits ? units + room + 7 : 0) / 8 * 8);
   x.partials = (int)(prefill ? 2 * x.slots : 2 * room);
+  const int alone = !prefill ? 64 : x.m == 256 ? 512 : 256;      // entries that a workgroup divides by itself
+  x.planned = x.entries > alone ? x.entries + (int)(room / heads) : 0;
   return x;
 }
 
 // The workspace: the fixed region of arrival counters (one per partial; at the same place for every shape, so that calls of
-// any shape may share it), then the partials.
-size_t attention_bytes(const Launch& x, int dim) { return kCounterBytes + (size_t)x.partials * x.m * (dim + 4) * 4; }
+// any shape may share it), then the partials, then the plan: two numbers, its pieces and its entries' tiles.
+size_t plan_at(const Launch& x, int dim) { return kCounterBytes + (size_t)x.partials * x.m * (dim + 4) * 4; }
+size_t attention_bytes(const Launch& x, int dim) {
+  return plan_at(x, dim) + (x.planned ? 32 + x.planned * sizeof(Planned) + (size_t)x.entries * 4 : 0);
+}
 
 }  // namespace
 }  // namespace xt
@@ -1750,6 +1815,8 @@ extern "C" int xt_page8_append(const void* k, int64_t k_row_stride, int64_t k_he
                k_pages, vt_pages, k_exp, v_exp, page_stride, head_stride, exp_page_stride, exp_head_stride, pages,
                page_shift_of(page_size), kv_heads, dim, table, table_stride, width, seq_lens, cu_rows, batch};
   const int64_t units = cu_rows ? rows / page_size + 2 * (int64_t)batch : batch;
+  if (units * (cu_rows ? 256 : 64) > 0xFFFFFFFFll)
+    return fail(XT_EUNSUPPORTED, "%s: %lld rows of %d requests in one call", what, (long long)rows, batch);
   const dim3 grid((unsigned)units, kv_heads, 2);
   const size_t lds = (size_t)dim * (page_size + 4);
   if (!cu_rows) append_kernel<64><<<grid, 64, lds, stream>>>(a);
@@ -1828,6 +1895,8 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
   const int64_t tiles = ((int64_t)width * page_size + kTile - 1) / kTile;    // of an entry at most
   if (tiles > 0x7FFFFFFF / x.entries || tiles * x.entries > ((int64_t)1 << 38) / kv_heads)
     return fail(XT_EUNSUPPORTED, "%s: %d row tiles over a table of %d pages", what, x.entries, width);
+  if ((int64_t)x.entries * kv_heads >= kMaxUnits)
+    return fail(XT_EUNSUPPORTED, "%s: %d row tiles of %d KV heads in one call", what, x.entries, kv_heads);
   if (x.partials > kCounterSlots)
     return fail(XT_EUNSUPPORTED, "%s: %d KV heads, at most %d", what, kv_heads, kCounterSlots / 2);
   const size_t need = attention_bytes(x, dim);
@@ -1841,8 +1910,16 @@ extern "C" int xt_page8_attention(const void* q, int64_t q_row_stride, int64_t q
              group, table,
              table_stride, width, seq_lens, cu_q, batch, rows, window, sinks, scale * kLog2e, out, out_row_stride,
              out_head_stride, out_dtype == XT_DTYPE_BF16 ? 1 : 0, lse, x.entries, kMinTiles, x.slots,
-             (int32_t*)workspace, (float*)((uint8_t*)workspace + kCounterBytes), x.partials};
+             (int32_t*)workspace, (float*)((uint8_t*)workspace + kCounterBytes), x.partials, nullptr, nullptr, nullptr};
   const int m = x.m;
+  if (x.planned) {
+    a.plan = (int*)((uint8_t*)workspace + plan_at(x, dim));
+    a.planned = (Planned*)(a.plan + 8);
+    a.plan_tiles = (int*)(a.planned + x.planned);
+    const int room = (m >= 128 ? groups : x.slots) / kv_heads;
+    plan_kernel<<<1, kPlanThreads, 0, stream>>>(a, m, room > 1 ? room : 1, m < 128);
+    if (const int st = check_launch(what)) return st;
+  }
   if (m == 16) {
     if (dim == 64) return launch_decode<64, 1>(what, a, groups, stream);
     if (dim == 128) return launch_decode<128, 1>(what, a, groups, stream);

@@ -351,6 +351,7 @@ extern "C" int xt_pages_free(int32_t* refs, int64_t pages, int32_t* table, int64
   if (const int st = check_table(what, refs, pages, table, table_stride, width, rows)) return st;
   if (n == 0) return ok();
   if (n < 0 || !lens || !which) return fail(XT_EINVAL, "%s: null pointer or negative count", what);
+  if (n > 0xFFFFFF) return fail(XT_EUNSUPPORTED, "%s: %d rows in one call", what, n);
   free_kernel<<<dim3(n, column_chunks(width)), 256, 0, stream>>>(refs, pages, table, table_stride, width, lens, rows,
                                                                  which);
   return check_launch(what);
