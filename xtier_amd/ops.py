@@ -1266,8 +1266,8 @@ def page8_attention(q, raw, table, seq_lens, scale, cu_q=None, window=0, sinks=0
     st = _lib.lib().xt_page8_attention(
         q.data_ptr(), qs[0], qs[1], *ptrs, q_heads, dim, page, *strides, table.data_ptr(), table.stride(0),
         table.shape[1], seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, rows,
-        min(int(window), _MAX_WINDOW), min(int(sinks), _MAX_WINDOW), float(scale), out.data_ptr(), os[0], os[1], out_dtype, None if lse is None else lse.data_ptr(),
-        ws.data_ptr(), ws.numel(), _stream(q))
+        min(int(window), _MAX_WINDOW), min(int(sinks), _MAX_WINDOW), float(scale), out.data_ptr(), os[0], os[1],
+        out_dtype, None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(q))
     if st:
         _lib.check(st, 'page8_attention')
     return out
