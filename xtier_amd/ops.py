@@ -1160,7 +1160,8 @@ def _check_page8(what, raw):
     shape, ks, es = k.shape, k.stride(), k_exp.stride()
     if len(shape) == 4:
         pages, heads, page, dim = shape
-        if (ks[3] == 1 and ks[2] == dim and min(ks[0], ks[1], es[0], es[1]) > 0 and vt.shape == (pages, heads, dim, page) and k_exp.shape == shape[:2]
+        if (ks[3] == 1 and ks[2] == dim and min(ks[0], ks[1], es[0], es[1]) > 0
+                and vt.shape == (pages, heads, dim, page) and k_exp.shape == shape[:2]
                 and vt.stride() == (ks[0], ks[1], page, 1) and v_exp.shape == shape[:2] and v_exp.stride() == es
                 and k.dtype in _E4M3_BYTES and vt.dtype in _E4M3_BYTES and k_exp.dtype is torch.uint8
                 and v_exp.dtype is torch.uint8):
@@ -1392,7 +1393,8 @@ def pages_copy(buffers, moves, count=None):
     if not isinstance(buffers, PageBuffers):
         buffers = PageBuffers(buffers)
     if moves.dim() != 2 or moves.shape[0] != 2 or moves.dtype is not torch.int32 \
-            or (moves.shape[1] > 1 and moves.stride(1) != 1) or (count is not None and (count.dtype is not torch.int32 or count.numel() != 1)):
+            or (moves.shape[1] > 1 and moves.stride(1) != 1) \
+            or (count is not None and (count.dtype is not torch.int32 or count.numel() != 1)):
         raise ValueError('xtier_amd.pages_copy: int32 moves [2, n] and an int32 count expected')
     away = _away('pages_copy', moves, count, *buffers.tensors[:1])
     if away is not None:
