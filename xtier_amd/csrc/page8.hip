@@ -777,70 +777,73 @@ __device__ inline float lse_of(float m, float l) {
   return l != 0.0f ? (m + __builtin_log2f(l)) * kLn2 : -__builtin_inff();
 }
 
+// A partial's maximum and sum, read as load_partial reads.
+__device__ inline float2_t load_max_sum(__amdgpu_buffer_rsrc_t r, int byte_off) {
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+  const u32x2_t w = __builtin_amdgcn_raw_buffer_load_b64(r, byte_off, 0, 17 /* sc0 sc1 */);
+  const uint32_t m = w[0], l = w[1];
+  return float2_t{__uint_as_float(m), __uint_as_float(l)};
+}
+
 // The last workgroup of a (head, entry) merges its partials, slots of [rows][D O values, max, sum, padding]: normalized
 // outputs, their maximum (of scaled scores in base 2) and their sum relative to it. slot_of(i): the i-th one's slot.
-// Reads miss every cache, so a thread has those of UB pieces of CB workgroups in flight at once.
+// Reads miss every cache, and what the merge takes is their round trips, so a thread has UB pieces of a row, of CB
+// workgroups, in flight at once, with one maximum and sum of each. (A maximum and sum for each piece left room for half as
+// much: 1 request, 2 KV heads x 256, 4099 keys, 16.7 us and 15.0 now; 2 requests of 80 rows at 63K 219 and 136. Sharing
+// them through LDS, loaded 16 workgroups side by side, was slower than either: 520.)
 template <int D, int M, int T, int UB, int CB, typename SlotOf>
 __device__ inline void merge_partials(const AttnArgs& a, const Entry& en, int head, SlotOf slot_of, int sharers,
                                       __amdgpu_buffer_rsrc_t pr) {
-  constexpr int kPieces = D / 4, kPitch = D + 4, kSlot = M * kPitch;
-  const int units = (en.r1 - en.r0) * kPieces;
-  for (int i0 = (int)threadIdx.x; i0 < units; i0 += T * UB) {
-    float mx[UB], l[UB];
+  constexpr int kPer = D / 4 / UB, kPitch = D + 4, kSlot = M * kPitch;    // threads of a row
+  const int units = (en.r1 - en.r0) * kPer;
+  for (int i = (int)threadIdx.x; i < units; i += T) {
+    const int row = i / kPer, d = i % kPer * 4;
+    float mx = -__builtin_inff(), l = 0.0f;
     float4_t o[UB];
 #pragma unroll
-    for (int k = 0; k < UB; ++k) {
-      mx[k] = -__builtin_inff();
-      l[k] = 0.0f;
-      o[k] = float4_t{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int k = 0; k < UB; ++k) o[k] = float4_t{0.f, 0.f, 0.f, 0.f};
     for (int w0 = 0; w0 < sharers; w0 += CB) {
-      float4_t ml[UB][CB], x[UB][CB];
+      float2_t ml[CB];
+      float4_t x[UB][CB];
 #pragma unroll
-      for (int k = 0; k < UB; ++k)
+      for (int c = 0; c < CB; ++c) {
+        // (past the last workgroup: an offset past the buffer, which reads zeros)
+        const bool real = w0 + c < sharers;
+        const int at = real ? (slot_of(w0 + c) * kSlot + row * kPitch) * 4 : -16 - 4 * D;
+        ml[c] = load_max_sum(pr, at + 4 * D);
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-          const int w = w0 + c;
-          const int i = i0 + k * T;
-          // (past the last workgroup or piece: an offset past the buffer, which reads zeros)
-          const bool real = w < sharers && i < units;
-          const int at = real ? (slot_of(w) * kSlot + i / kPieces * kPitch) * 4 : -16;
-          ml[k][c] = load_partial(pr, real ? at + 4 * D : -16);
-          x[k][c] = load_partial(pr, real ? at + i % kPieces * 16 : -16);
-          if (!real) ml[k][c][0] = -__builtin_inff();
-        }
+        for (int k = 0; k < UB; ++k) x[k][c] = load_partial(pr, at + 4 * (d + 4 * kPer * k));
+      }
+      float m = mx;
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        if (w0 + c >= sharers) ml[c][0] = -__builtin_inff();
+        m = fmaxf(m, ml[c][0]);
+      }
+      const float mu = m == -__builtin_inff() ? 0.0f : m;
+      // shares of the sum, so that o stays a convex combination
+      float wt[CB];
+      const float old = l * __builtin_amdgcn_exp2f(mx - mu);
+      float sum = old;
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        wt[c] = ml[c][1] * __builtin_amdgcn_exp2f(ml[c][0] - mu);
+        sum += wt[c];
+      }
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
       for (int k = 0; k < UB; ++k) {
-        float m = mx[k];
-#pragma unroll
-        for (int c = 0; c < CB; ++c) m = fmaxf(m, ml[k][c][0]);
-        const float mu = m == -__builtin_inff() ? 0.0f : m;
-        // shares of the sum, so that o stays a convex combination
-        float wt[CB];
-        const float old = l[k] * __builtin_amdgcn_exp2f(mx[k] - mu);
-        float sum = old;
-#pragma unroll
-        for (int c = 0; c < CB; ++c) {
-          wt[c] = ml[k][c][1] * __builtin_amdgcn_exp2f(ml[k][c][0] - mu);
-          sum += wt[c];
-        }
-        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
         o[k] *= old * inv;
 #pragma unroll
         for (int c = 0; c < CB; ++c) o[k] += wt[c] * inv * x[k][c];
-        l[k] = sum;
-        mx[k] = m;
       }
+      l = sum;
+      mx = m;
     }
+    const int r = en.r0 + row, tok = r / a.group, qh = head * a.group + r % a.group;
 #pragma unroll
-    for (int k = 0; k < UB; ++k) {
-      const int i = i0 + k * T;
-      if (i >= units) continue;
-      const int r = en.r0 + i / kPieces, d = i % kPieces * 4;
-      const int tok = r / a.group, qh = head * a.group + r % a.group;
-      store_out(a, en.row0 + tok, qh, d, o[k]);
-      if (a.lse && d == 0) a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] = lse_of(mx[k], l[k]);
-    }
+    for (int k = 0; k < UB; ++k) store_out(a, en.row0 + tok, qh, d + 4 * kPer * k, o[k]);
+    if (a.lse && d == 0) a.lse[(int64_t)(en.row0 + tok) * a.heads * a.group + qh] = lse_of(mx, l);
   }
 }
 
@@ -1212,7 +1215,7 @@ __global__ __launch_bounds__(256, decode_per_cu(D)) void decode_kernel(AttnArgs 
       const int first = pc.slot - pc.at;
       int32_t* counter = a.counters + first;
       if (arrive_last(counter, pc.count, &s_last)) {
-        merge_partials<D, M, 256, D == 256 ? 2 : 1, 16>(a, en, head, [&](int i) { return first + i; }, pc.count, pr);
+        merge_partials<D, M, 256, D / 64, 16>(a, en, head, [&](int i) { return first + i; }, pc.count, pr);
         reset_counter(counter);
       }
     }
@@ -1692,7 +1695,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && W == 4 ? 1 : 2) void prefill_ke
     if (!alone) {
       int32_t* counter = a.counters + sg.counter;
       if (arrive_last(counter, sg.sharers, &s_last)) {
-        merge_partials<D, M, T, 4, 4>(a, en, head, [&](int i) { return sg.slot(i); }, sg.sharers, pr);
+        merge_partials<D, M, T, 4, 8>(a, en, head, [&](int i) { return sg.slot(i); }, sg.sharers, pr);
         reset_counter(counter);
       }
     }
