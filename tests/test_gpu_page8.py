@@ -43,12 +43,24 @@ def _check_append(raw, table, lens, cu, k, v, page, pass_cu=True):
     _same_pool(pool, raw)
 
 
-@pytest.mark.parametrize('page,heads,dim', [(16, 2, 64), (32, 1, 256), (64, 4, 128), (128, 3, 64), (128, 1, 256)])
+@pytest.mark.parametrize('page,heads,dim', [(16, 2, 64), (32, 1, 256), (64, 4, 128), (128, 3, 64), (128, 2, 128),
+                                            (128, 1, 256)])
 def test_append_ragged_requests(page, heads, dim):
     rng = np.random.default_rng(page + dim)
     old = [0, 5, page - 1, page, 2 * page + 3, 0, 7]
     new = [1, page + 2, 1, 3 * page + 5, 0, 2 * page, page - 7]
     _check_append(*_append_case(rng, old, new, page, heads, dim), page)
+
+
+def test_append_many_requests():
+    """More requests than lanes of a wave, and than 64 times 64, some without rows, the first one's rows not at 0."""
+    rng = np.random.default_rng(37)
+    for n, page in ((65, 16), (700, 32), (4200, 16)):
+        old, new = rng.integers(0, 40, n).tolist(), rng.integers(0, 4, n).tolist()
+        new[n // 2], new[0] = 90, 0
+        raw, table, lens, cu, k, v = _append_case(rng, old, new, page, 1, 64)
+        _check_append(raw, table, lens, cu, k, v, page)
+        _check_append(raw, table[n // 2 + 1:], lens[n // 2 + 1:], cu[n // 2 + 1:], k, v, page)
 
 
 @pytest.mark.parametrize('page,heads,dim', [(16, 4, 64), (64, 4, 128), (128, 2, 256)])

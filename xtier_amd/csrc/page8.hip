@@ -72,8 +72,8 @@ __device__ inline uint32_t e4m3_pair(float a, float b) {
 // One workgroup per (touched page, head, K or V). A thread keeps its first kKeep 16-byte pieces of the new rows in
 // registers between the largest magnitude and the conversion; of larger pages the rest is read again, from L2. The rows'
 // addresses do not depend on the page, so their loads go out before the table's answer is in. V is transposed through
-// LDS. Bound by the chain of loads and the launch: measured 4.5 us for one row each of 32 requests (4 heads
-// x 128), 9.3 for a chunk of 4096, 8.8 for 24 requests of up to 300 (2 x 256, pages of 16).
+// LDS. Bound by the chain of loads and the launch: measured 4.0 us for one row each of 32 requests (4 heads
+// x 128), 8.5 for a chunk of 4096, 8.8 for 24 requests of up to 300 (2 x 256, pages of 16).
 constexpr int kKeep = 4;
 
 template <int T>
@@ -92,12 +92,16 @@ __global__ __launch_bounds__(T) void append_kernel(AppendArgs a) {
     row0 = b;
     n = 1;
   } else {
-    // request b's units start at floor(cu[b] / page) + 2 b: n rows touch at most floor(n / page) + 2 pages
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((a.cu_rows[mid] >> a.page_shift) + 2 * (int64_t)mid <= unit) lo = mid;
-      else hi = mid - 1;
+    // request b's units start at floor(cu[b] / page) + 2 b: n rows touch at most floor(n / page) + 2 pages. The last
+    // request that starts at or before this unit, 64 candidates at a time (every wave alike).
+    int lo = 0;
+    for (int n_left = a.batch; n_left > 1;) {
+      const int step = (n_left + 63) / 64, off = (tid & 63) * step;
+      const bool here = off < n_left && (a.cu_rows[lo + off] >> a.page_shift) + 2 * (int64_t)(lo + off) <= unit;
+      const int found = (int)__popcll(__ballot(here));     // (unsigned; none: a unit before the first request's)
+      const int k = found > 0 ? (found - 1) * step : 0;
+      lo += k;
+      n_left = min(step, n_left - k);
     }
     b = lo;
     row0 = a.cu_rows[b];
@@ -1818,12 +1822,18 @@ extern "C" int xt_page8_append(const void* k, int64_t k_row_stride, int64_t k_he
                k_pages, vt_pages, k_exp, v_exp, page_stride, head_stride, exp_page_stride, exp_head_stride, pages,
                page_shift_of(page_size), kv_heads, dim, table, table_stride, width, seq_lens, cu_rows, batch};
   const int64_t units = cu_rows ? rows / page_size + 2 * (int64_t)batch : batch;
-  if (units * (cu_rows ? 256 : 64) > 0xFFFFFFFFll)
+  if (units * 1024 > 0xFFFFFFFFll)
     return fail(XT_EUNSUPPORTED, "%s: %lld rows of %d requests in one call", what, (long long)rows, batch);
   const dim3 grid((unsigned)units, kv_heads, 2);
   const size_t lds = (size_t)dim * (page_size + 4);
-  if (!cu_rows) append_kernel<64><<<grid, 64, lds, stream>>>(a);
-  else append_kernel<256><<<grid, 256, lds, stream>>>(a);
+  // as many threads as keep a page's new rows, those that a request brings on average, in registers: 610 requests of up to 5
+  // rows, 4 heads x 64, 27 us with 256 threads and 10 with 64; 574 rows, 4 x 256, pages of 128, 17 with 256 and 10 with
+  // 1024; 8 x 1024 rows, 4 x 128, pages of 128, 14.4 with 256, 12.7 with 512, 15.8 with 1024
+  const int64_t pieces = (rows < (int64_t)batch * page_size ? (rows + batch - 1) / batch : page_size) * (dim / 8);
+  if (pieces <= 64 * kKeep) append_kernel<64><<<grid, 64, lds, stream>>>(a);
+  else if (pieces <= 256 * kKeep) append_kernel<256><<<grid, 256, lds, stream>>>(a);
+  else if (pieces <= 512 * kKeep) append_kernel<512><<<grid, 512, lds, stream>>>(a);
+  else append_kernel<1024><<<grid, 1024, lds, stream>>>(a);
   return check_launch(what);
 }
 
