@@ -361,6 +361,25 @@ def test_large_batches(dim, heads, group, n, most, window):
     _check_attention(raw, table, lens, cu, q, 16, window, 3 if window else 0, large=True)
 
 
+@pytest.mark.parametrize('n,most', [(12, 3), (90, 3), (8, 60), (560, 30)])
+def test_rows_before_the_first_request(n, most):
+    """Offsets that do not begin at 0: the rows before them are left as they are, whichever way the work is divided."""
+    rng = np.random.default_rng(38 + n)
+    rows = rng.integers(1, most + 1, n)
+    lens = rows + rng.integers(0, 60, n)
+    raw, table, lens, cu, q = _attention_case(rng, lens.tolist(), rows.tolist(), 16, 1, 8, 128)
+    s = n // 4
+    at = int(cu[s])
+    out = torch.full(q.shape, 5.0, dtype=torch.bfloat16, device='cuda')
+    pool = gpu_raw(raw)
+    pool.attend(q.cuda(), torch.from_numpy(table[s:]).cuda(), torch.from_numpy(lens[s:]).cuda(), 0.01,
+                torch.from_numpy(cu[s:]).cuda(), out=out)
+    ref, lse, spread, score = attention_on_gpu(q[at:], raw, table[s:], 16, lens[s:], 0.01, cu[s:] - cu[s])
+    tol, _ = attention_tolerance(ref, lse, spread, score, raw, int(lens.max()), 128, 2.0 ** -7)
+    assert at > 0 and (out[:at] == 5).all()
+    assert (np.abs(out[at:].double().cpu().numpy() - ref) <= tol).all()
+
+
 def test_a_large_batch_in_a_graph():
     """A replay follows lengths that changed, where a plan is made on the device too."""
     rng = np.random.default_rng(36)
