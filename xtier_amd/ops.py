@@ -1161,8 +1161,8 @@ def _check_page8(what, raw):
     if len(shape) == 4:
         pages, heads, page, dim = shape
         if (ks[3] == 1 and ks[2] == dim and min(ks[0], ks[1], es[0], es[1]) > 0
-                and vt.shape == (pages, heads, dim, page) and k_exp.shape == shape[:2]
-                and vt.stride() == (ks[0], ks[1], page, 1) and v_exp.shape == shape[:2] and v_exp.stride() == es
+                and vt.shape == (pages, heads, dim, page) and k_exp.shape == (pages, heads)
+                and vt.stride() == (ks[0], ks[1], page, 1) and v_exp.shape == (pages, heads) and v_exp.stride() == es
                 and k.dtype in _E4M3_BYTES and vt.dtype in _E4M3_BYTES and k_exp.dtype is torch.uint8
                 and v_exp.dtype is torch.uint8):
             return ((k.data_ptr(), vt.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), pages, heads), dim, page,
